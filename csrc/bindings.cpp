@@ -60,6 +60,15 @@ void gdn_gates(torch::Tensor a, torch::Tensor b, torch::Tensor A_log, torch::Ten
 void causal_conv1d(torch::Tensor x, torch::Tensor window, torch::Tensor w, c10::optional<torch::Tensor> bias,
                    torch::Tensor tok_start, torch::Tensor slot, c10::optional<torch::Tensor> n_commit, torch::Tensor y);
 void gated_rmsnorm(torch::Tensor o, torch::Tensor z, torch::Tensor w, double eps, torch::Tensor y);
+void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g, torch::Tensor beta,
+                 torch::Tensor state, torch::Tensor tok_start, torch::Tensor slot, double scale, torch::Tensor out,
+                 torch::Tensor status);
+void qk_norm_rope_kv_write(torch::Tensor qkv, torch::Tensor wq, torch::Tensor wk, double eps, torch::Tensor pos,
+                           c10::optional<torch::Tensor> slots, torch::Tensor cos_sin, torch::Tensor q_out,
+                           c10::optional<torch::Tensor> k_cache, c10::optional<torch::Tensor> v_cache, int64_t Hq,
+                           int64_t Hkv, int64_t D, torch::Tensor status);
+void spec_verify_probs(torch::Tensor p, c10::optional<torch::Tensor> q, torch::Tensor tokens, torch::Tensor coins,
+                       c10::optional<torch::Tensor> n_draft, torch::Tensor acc, torch::Tensor bonus);
 torch::Tensor raster(torch::Tensor tris, torch::Tensor cols, torch::Tensor vp, int64_t W, int64_t H,
                      std::vector<double> light, double ambient, double diffuse, double exposure, std::vector<double> bg);
 void sample_candidates(torch::Tensor logits, int64_t kc, c10::optional<torch::Tensor> temp, int64_t rows_per_temp,
@@ -97,6 +106,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gdn_gates", &phx::gdn_gates);
   m.def("causal_conv1d", &phx::causal_conv1d);
   m.def("gated_rmsnorm", &phx::gated_rmsnorm);
+  m.def("gdn_chunked", &phx::gdn_chunked);
+  m.def("qk_norm_rope_kv_write", &phx::qk_norm_rope_kv_write);
+  m.def("spec_verify_probs", &phx::spec_verify_probs);
   m.def("raster", &phx::raster);
   m.def("raster_pbr", &phx::raster_pbr);
   m.def("sample_candidates", &phx::sample_candidates);

@@ -140,6 +140,48 @@ def tree_accept_reference(logits, tokens: torch.Tensor, parent: torch.Tensor, te
     return acc, bonus
 
 
+def chain_reject_reference(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor,
+                           coins: torch.Tensor, n_draft: Optional[torch.Tensor] = None
+                           ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Speculative sampling of draft chains (the definition of ops.spec_verify_probs, whose arguments it takes).
+
+    Draft x_d ~ q_d is kept iff u_d q_d(x_d) < p_d(x_d); the first one that is not is replaced by a draw from
+    max(p_d - q_d, 0), renormalised (from p_d if that is empty), and after n kept drafts the bonus is drawn from
+    p_{n+1}: every emitted token then follows p exactly. NaN and negative weights count as 0."""
+    R, D = tokens.shape
+    if target.dim() != 3 or target.shape[:2] != (R, D + 1) or coins.shape != (R, D + 2):
+        raise ValueError("chain verification: target [R, D + 1, V], tokens [R, D], coins [R, D + 2]")
+    if draft is not None and (draft.shape != (R, D, target.shape[2]) or draft.dtype != target.dtype):
+        raise ValueError("chain verification: draft probabilities [R, D, V] of the target's type")
+    V = target.shape[2]
+    acc = torch.full((R, D), -1, dtype=torch.int64, device=tokens.device)
+    bonus = torch.zeros(R, dtype=torch.int64, device=tokens.device)
+    for r in range(R):
+        n = D if n_draft is None else min(max(int(n_draft[r]), 0), D)
+        k = 0
+        while k < n:
+            x = int(tokens[r, k])
+            if not 0 <= x < V:
+                break
+            q = 1.0 if draft is None else float(draft[r, k, x])
+            if not float(coins[r, k]) * q < float(target[r, k, x]):
+                break
+            acc[r, k] = k + 1
+            k += 1
+        p = torch.nan_to_num(target[r, k].double(), nan=0.0).clamp(min=0)
+        rest = p
+        if k < n:
+            if draft is not None:
+                rest = torch.nan_to_num(target[r, k].double() - draft[r, k].double(), nan=0.0).clamp(min=0)
+            elif 0 <= int(tokens[r, k]) < V:
+                rest = p.clone()
+                rest[int(tokens[r, k])] = 0.0
+            if float(rest.sum()) <= 0:
+                rest = p
+        bonus[r] = sample_from(rest[None], coins[r, D + 1:])[0]
+    return acc, bonus
+
+
 def sample_from(probs: torch.Tensor, coin: torch.Tensor) -> torch.Tensor:
     """Inverse-CDF draw: first index whose cumulative mass exceeds coin (coins in [0,1))."""
     cum = torch.cumsum(probs.double(), dim=-1)

@@ -31,7 +31,8 @@ _STATUS = {}
 STATUS_CODES = {1: "timeout in TMA producer", 2: "timeout in MMA issuer", 3: "timeout in epilogue",
                 4: "timeout waiting for a peer rank", 5: "bad arguments",
                 6: "fp8 block scale is not a power of two (hardware-scaled GEMM)",
-                7: "timeout in a split-K GEMM part waiting for the other parts of its tile"}
+                7: "timeout in a split-K GEMM part waiting for the other parts of its tile",
+                8: "a token range, slot or position outside its buffer"}
 
 
 _LAUNCHES = [0]
@@ -349,6 +350,29 @@ def spec_sample_accept(logits: torch.Tensor, tokens: torch.Tensor, parent: torch
     return acc, bonus
 
 
+def spec_verify_probs(target_probs: torch.Tensor, draft_probs: Optional[torch.Tensor], tokens: torch.Tensor,
+                      coins: torch.Tensor, n_draft: Optional[torch.Tensor] = None):
+    """Verify sampled draft chains by rejection (csrc/spec_verify.cu). target_probs [R, D + 1, V] (fp32, bf16 or
+    fp16; row d: the target's distribution where draft d stands, row D after all of them), draft_probs [R, D, V]
+    of the same type (the distributions the drafts were drawn from; None: greedy drafts, one at their token),
+    tokens [R, D] int64, coins [R, D + 2] fp32 in [0, 1) (column d for draft d, column D + 1 for the bonus draw: the
+    layout of engine.sampling.seeded_coins), n_draft [R] int32: drafts of each request (None: D). Draft d is kept iff
+    coin * q(x) < p(x); the first one that is not is replaced by a draw from max(p - q, 0), and if all are kept the
+    bonus is a draw from the next row of p. With D = 0 this is a plain draw from given probabilities. A row without
+    any mass gives index V - 1. Returns (accepted node ids [R, D] int64: node d + 1 for draft d, -1 padded; bonus
+    tokens [R] int64), as spec_sample_accept does."""
+    R, D = tokens.shape
+    if _check.active():
+        _check.spec_verify_probs(target_probs, draft_probs, tokens, coins, n_draft)
+    if target_probs.is_cuda:
+        acc = torch.empty(R, D, dtype=torch.int64, device=target_probs.device)
+        bonus = torch.empty(R, dtype=torch.int64, device=target_probs.device)
+        ext().spec_verify_probs(target_probs, draft_probs, tokens.contiguous(), coins.contiguous(), n_draft, acc, bonus)
+        return acc, bonus
+    from ..engine.sampling import chain_reject_reference
+    return chain_reject_reference(target_probs, draft_probs, tokens, coins, n_draft)
+
+
 # ------------------------------------------------------------------------------------------------
 # norms / activations / quant
 # ------------------------------------------------------------------------------------------------
@@ -464,6 +488,43 @@ def rope_kv_write(qkv: torch.Tensor, pos: torch.Tensor, slots: Optional[torch.Te
         pg, off = sl // page_size, sl % page_size
         k_cache[pg, :, off, :] = rot(k[ok], ok).to(k_cache.dtype)
         v_cache[pg, :, off, :] = v[ok].to(v_cache.dtype)
+    return q_out
+
+
+def qk_norm_rope_kv_write(qkv: torch.Tensor, wq: torch.Tensor, wk: torch.Tensor, eps: float, pos: torch.Tensor,
+                          slots: Optional[torch.Tensor], cos_sin: torch.Tensor, k_cache: Optional[torch.Tensor],
+                          v_cache: Optional[torch.Tensor], hq: int, hkv: int, d: int,
+                          q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """rope_kv_write for models that norm their q and k heads: RMS norm of every q head (weight wq [d]) and k head
+    (wk [d]), then the rotation, in one pass with one rounding (csrc/qk_norm.cu). cos_sin [positions, rot / 2, 2] may
+    cover only the first rot elements of a head (partial rotation); the others are normed. Rows with slot -1 get their
+    q and write nothing to the cache."""
+    m = qkv.shape[0]
+    if q_out is None:
+        q_out = torch.empty(m, hq, d, dtype=qkv.dtype, device=qkv.device)
+    if _check.active():
+        _check.qk_norm_rope_kv_write(qkv, wq, wk, pos, slots, cos_sin, k_cache, hq, hkv, d)
+    if qkv.is_cuda:
+        ext().qk_norm_rope_kv_write(qkv, wq, wk, eps, pos, slots, cos_sin, q_out, k_cache, v_cache, hq, hkv, d,
+                                    status_tensor(qkv.device))
+        return q_out
+    if qkv.shape[1] != (hq + 2 * hkv) * d or wq.numel() != d or wk.numel() != d or 2 * cos_sin.shape[1] > d:
+        raise ValueError("qk_norm_rope_kv_write: qkv [m, (hq + 2 hkv) d], norm weights [d], a table of at most d / 2 pairs")
+    x = qkv.float().view(m, hq + 2 * hkv, d)
+    w = torch.cat([wq.float().expand(hq, d), wk.float().expand(hkv, d)])
+    y = x[:, :hq + hkv]
+    y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w
+    half = cos_sin.shape[1]
+    c, s = cos_sin[pos.long()][:, None].unbind(-1)
+    y1, y2 = y[..., :half], y[..., half:2 * half]
+    y = torch.cat([y1 * c - y2 * s, y2 * c + y1 * s, y[..., 2 * half:]], -1)
+    q_out.copy_(y[:, :hq])
+    if k_cache is not None and slots is not None:
+        ok = slots >= 0
+        sl = slots[ok].long()
+        pg, off = sl // k_cache.shape[2], sl % k_cache.shape[2]
+        k_cache[pg, :, off, :] = y[ok, hq:].to(k_cache.dtype)
+        v_cache[pg, :, off, :] = x[ok, hq + hkv:].to(v_cache.dtype)
     return q_out
 
 

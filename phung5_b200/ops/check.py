@@ -196,6 +196,46 @@ def spec_sample_accept(logits, tokens, parent, top_k, temp, depth: int, kc: int,
     _range(op, "tokens (drafts)", tokens[:, 1:], 0, 1 << 31)
 
 
+def spec_verify_probs(target, draft, tokens, coins, n_draft) -> None:
+    op = "spec_verify_probs"
+    R, D = tokens.shape
+    if target.dim() != 3 or tuple(target.shape[:2]) != (R, D + 1):
+        _fail(op, f"target_probs has shape {tuple(target.shape)}, expected ({R}, {D + 1}, V)")
+    if draft is not None:
+        _shape(op, "draft_probs", draft, (R, D, target.shape[2]))
+    _shape(op, "coins", coins, (R, D + 2))
+    if bool(((coins < 0) | (coins >= 1) | coins.isnan()).any()):
+        _fail(op, "coins must lie in [0, 1)")
+    drafts = tokens
+    if n_draft is not None:
+        _range(op, "n_draft", n_draft, 0, D + 1)
+        drafts = tokens[torch.arange(D, device=tokens.device)[None] < n_draft[:, None]]
+    _range(op, "tokens (drafts)", drafts, 0, target.shape[2])
+
+
+def gdn_chunked(q, k, v, g, beta, state, tok_start, slot) -> None:
+    op = "gdn_chunked"
+    t, hv = v.shape[0], v.shape[1]
+    for name, x in (("g", g), ("beta", beta)):
+        _shape(op, name, x, (t, hv))
+    _shape(op, "state", state, (state.shape[0], hv, 128, 128))
+    if tok_start.numel() != slot.numel() + 1:
+        _fail(op, f"tok_start has {tok_start.numel()} entries for {slot.numel()} requests")
+    _range(op, "tok_start", tok_start, 0, t + 1)
+    _nondecreasing(op, "tok_start", tok_start)
+    _range(op, "slot", slot, 0, state.shape[0])
+    _distinct(op, "slot", slot)
+
+
+def qk_norm_rope_kv_write(qkv, wq, wk, pos, slots, cos_sin, k_cache, hq: int, hkv: int, d: int) -> None:
+    op = "qk_norm_rope_kv_write"
+    for name, w in (("wq", wq), ("wk", wk)):
+        _shape(op, name, w, (d,))
+    if 2 * cos_sin.shape[1] > d:
+        _fail(op, f"the table rotates {2 * cos_sin.shape[1]} of {d} elements")
+    rope_kv_write(qkv, pos, slots, cos_sin, k_cache, hq, hkv, d)
+
+
 def rope_kv_write(qkv, pos, slots, cos_sin, k_cache, hq: int, hkv: int, d: int) -> None:
     op = "rope_kv_write"
     m = qkv.shape[0]

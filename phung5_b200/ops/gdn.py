@@ -11,6 +11,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from . import check as _check
 from . import ext, status_tensor  # noqa: F401
 
 
@@ -62,6 +63,30 @@ def gdn_recurrent(q, k, v, g, beta, state, tok_start, slot, scale: float, write_
         if write_state:
             state[int(slot[r])] = S
     return out, st
+
+
+def gdn_chunked(q, k, v, g, beta, state, tok_start, slot, scale: float, out: Optional[torch.Tensor] = None):
+    """The recurrence of gdn_recurrent(write_state=True) for prompt passes (csrc/gdn_chunk.cu): q, k [T, HK, 128] and
+    v [T, HV, 128] bf16 (strided views are taken as they are), g, beta [T, HV] fp32, state [slots, HV, 128, 128] fp32,
+    advanced in place at slot[r] over tokens [tok_start[r], tok_start[r + 1]); requests without tokens keep their
+    state. Returns out [T, HV, 128]; rows outside every request are not written."""
+    if _check.active():
+        _check.gdn_chunked(q, k, v, g, beta, state, tok_start, slot)
+    if q.is_cuda:
+        if out is None:
+            out = torch.empty(v.shape, dtype=torch.bfloat16, device=v.device)
+        ext().gdn_chunked(q, k, v, g.contiguous(), beta.contiguous(), state, tok_start, slot, scale, out,
+                          status_tensor(q.device))
+        return out
+    if q.shape != k.shape or q.shape[2] != 128 or v.shape[2] != 128 or q.shape[0] != v.shape[0] or \
+            v.shape[1] % q.shape[1] or tok_start.numel() != slot.numel() + 1:
+        raise ValueError("gdn_chunked: q, k [T, HK, 128], v [T, HV, 128], HV a multiple of HK, tok_start [R + 1], slot [R]")
+    o, _ = gdn_recurrent(q, k, v, g, beta, state, tok_start, slot, scale, write_state=True, stash=False)
+    if out is None:
+        return o
+    a, b = int(tok_start[0]), int(tok_start[-1])
+    out[a:b] = o[a:b]
+    return out
 
 
 def gdn_fold(state, tok_start, slot, n_accept, st) -> None:
