@@ -10,6 +10,7 @@
 #include <torch/extension.h>
 
 #include "common.cuh"
+#include "tmap.h"
 
 namespace phx {
 
@@ -39,6 +40,7 @@ __device__ __forceinline__ bool request(const GdnArgs& a, int r, int& t0, int& t
   return ok;
 }
 
+constexpr int kStepMean = 16;            // mean tokens per request up to which tokens are taken one by one
 constexpr int kStepTokens = 16;          // tokens whose q and k are normalised together
 constexpr int kHalf = kDim / 2;
 constexpr int kRowPad = kDim + 8;        // the second half starts 4 floats later: both halves' reads miss each other's banks
@@ -123,6 +125,549 @@ __global__ void __launch_bounds__(256) gdn_step_kernel(const GdnArgs a) {
   for (int i = 0; i < kHalf; ++i) S[i * kDim] = col[i];
 }
 
+// ------------------------------------------------------------------------------------------------
+// Chunks of 64 tokens. With b_i the sum of g up to token i of a chunk, S0 the state before it:
+//   (I + L) V' = diag(beta) (V - diag(e^b) K^ S0),   L_ij = beta_i e^(b_i - b_j) k^_i . k^_j   (j < i)
+//   O  = diag(e^b) Q^ S0 + P V',                     P_ij = e^(b_i - b_j) q^_i . k^_j          (j <= i)
+//   S1 = e^(b_C) S0 + sum_j e^(b_C - b_j) k^_j v'_j^T
+// gdn_prep_kernel forms X = (I + L)^-1 - I, P and the tokens' factors for every chunk and head at once; gdn_chain_kernel
+// walks the chunks of one (request, head) with the state in registers. The normalisation of k and q is folded into
+// those factors, so the tensor core reads k and q as they are in memory (bf16, exact); every fp32 operand (S, X, P and
+// the two right-hand sides) goes in as two bf16 pieces, hi = bf16(x) and lo = bf16(x - hi), off by at most 2^-18 of x.
+// ------------------------------------------------------------------------------------------------
+constexpr int kC = 64;                                   // tokens per chunk
+constexpr int kTri = 5120;                               // one piece of a lower-triangular 64 x 64 matrix, see tri_offset
+constexpr int kVecFloats = 4 * kC + 16;                  // beta, c1, c2, c3 per token; e^(b_C)
+constexpr int kItemBytes = 4 * kTri + kVecFloats * 4;    // X hi, X lo, P hi, P lo, factors
+
+// Bytes from the start of a piece to element (i, j), j / 16 <= i / 16. The 16-column step s = j / 16 holds rows 16 s to
+// 63 as two columns of 8 x 16-byte core matrices (the tensor core's unswizzled K-major form), so the blocks above the
+// diagonal are neither stored nor multiplied.
+__host__ __device__ constexpr int tri_start(int s) { return 2048 * s - 256 * s * (s - 1); }
+__host__ __device__ constexpr int tri_offset(int i, int j) {
+  const int s = j / 16, rows = kC - 16 * s;
+  return tri_start(s) + (j % 16 / 8) * rows * 16 + (i - 16 * s) * 16 + (j % 8) * 2;
+}
+
+// Request r of work item w: items of request r start at tok_start[r] / 64 + r, which leaves each at least the
+// ceil(tokens / 64) it needs. At most T / 64 + R items in all.
+__device__ __forceinline__ int first_item(const GdnArgs& a, int r) { return a.tok_start[r] / kC + r; }
+
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(x0, x1);
+  lo = pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+}
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+constexpr int kPrepRow = kDim + 8;     // bf16 elements of a padded shared row: ldmatrix's eight rows miss each other's banks
+constexpr int kLRow = kC + 4;
+struct PrepSmem {
+  union {
+    struct {
+      __nv_bfloat16 k[kC][kPrepRow], q[kC][kPrepRow];
+    } in;
+    uint8_t item[kItemBytes];          // the finished item, copied out in one go
+  };
+  float L[kC][kLRow];
+  float bh[kC], bl[kC];                // b as the sum of two floats: differences of far-down sums keep their digits
+  float rk[kC], rq[kC], beta[kC];
+};
+
+// One CTA per (work item, value head).
+__global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t* __restrict__ items) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  PrepSmem& s = *reinterpret_cast<PrepSmem*>(smem_raw);
+  const int w = blockIdx.x, h = blockIdx.y, hk = h / (a.HV / a.HK);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int lo = 0, hi = a.R - 1;            // the last request whose items start at or before w
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_item(a, mid) <= w) lo = mid;
+    else hi = mid - 1;
+  }
+  int t0, t1, slot;
+  if (!request(a, lo, t0, t1, slot)) return;
+  t0 += (w - first_item(a, lo)) * kC;
+  const int n = min(kC, t1 - t0);
+  if (n <= 0 || w < first_item(a, lo)) return;
+
+  // ---- q and k rows (zeros past the request's end), factors ----
+  for (int x = tid; x < kC * 16; x += 128) {
+    const int row = x >> 4, c = (x & 15) * 8;
+    uint4 kv = make_uint4(0, 0, 0, 0), qv = kv;
+    if (row < n) {
+      kv = *reinterpret_cast<const uint4*>(a.k + (int64_t)(t0 + row) * a.k_t + hk * a.k_h + c);
+      qv = *reinterpret_cast<const uint4*>(a.q + (int64_t)(t0 + row) * a.q_t + hk * a.q_h + c);
+    }
+    *reinterpret_cast<uint4*>(&s.in.k[row][c]) = kv;
+    *reinterpret_cast<uint4*>(&s.in.q[row][c]) = qv;
+  }
+  if (warp == 0) {
+    double b0 = 2 * lane < n ? a.g[(int64_t)(t0 + 2 * lane) * a.HV + h] : 0.f;
+    double b1 = b0 + (2 * lane + 1 < n ? a.g[(int64_t)(t0 + 2 * lane + 1) * a.HV + h] : 0.f);
+    double inc = b1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    b0 += inc - b1;
+    s.bh[2 * lane] = (float)b0, s.bl[2 * lane] = (float)(b0 - (float)b0);
+    s.bh[2 * lane + 1] = (float)inc, s.bl[2 * lane + 1] = (float)(inc - (float)inc);
+  } else if (warp < 3) {
+    const int i = tid - 32;
+    s.beta[i] = i < n ? a.beta[(int64_t)(t0 + i) * a.HV + h] : 0.f;
+  }
+  __syncthreads();
+  {
+    const int row = tid & 63;
+    const uint4* src = reinterpret_cast<const uint4*>(tid < 64 ? s.in.k[row] : s.in.q[row]);
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const uint4 u = src[c];
+      const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack_bf16x2(x[e]);
+        ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+      }
+    }
+    (tid < 64 ? s.rk : s.rq)[row] = rsqrtf(ss + 1e-6f) * (tid < 64 ? 1.f : a.scale);
+  }
+
+  // ---- Gram matrices k k^T and q k^T: warp w has rows 16 w .. 16 w + 15, columns up to the diagonal block ----
+  float kk[8][4], qk[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) kk[j][e] = qk[j][e] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) {
+    uint32_t ak[4], aq[4];
+    const int ar = warp * 16 + (lane & 15), ac = ks * 16 + (lane >> 4) * 8;
+    ldmatrix_x4(ak, smem_u32(&s.in.k[ar][ac]));
+    ldmatrix_x4(aq, smem_u32(&s.in.q[ar][ac]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {        // two column tiles of 8 at a time
+      if (j > warp) break;
+      uint32_t b[4];
+      ldmatrix_x4(b, smem_u32(&s.in.k[j * 16 + (lane >> 4) * 8 + (lane & 7)][ks * 16 + (lane >> 3 & 1) * 8]));
+      mma_bf16(kk[2 * j], ak, b[0], b[1]);
+      mma_bf16(kk[2 * j + 1], ak, b[2], b[3]);
+      mma_bf16(qk[2 * j], aq, b[0], b[1]);
+      mma_bf16(qk[2 * j + 1], aq, b[2], b[3]);
+    }
+  }
+  __syncthreads();     // the item's bytes take the place of k and q; the factors are complete
+  uint8_t* item = s.item;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j > 2 * warp + 1) break;
+#pragma unroll
+    for (int e2 = 0; e2 < 2; ++e2) {
+      const int i = warp * 16 + (lane >> 2) + 8 * e2, c = j * 8 + (lane & 3) * 2;
+      float l[2], p[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float d = c + e <= i ? expf((s.bh[i] - s.bh[c + e]) + (s.bl[i] - s.bl[c + e])) * s.rk[c + e] : 0.f;
+        l[e] = c + e < i ? kk[j][2 * e2 + e] * d * (s.beta[i] * s.rk[i]) : 0.f;
+        p[e] = c + e <= i ? qk[j][2 * e2 + e] * d * s.rq[i] : 0.f;
+      }
+      *reinterpret_cast<float2*>(&s.L[i][c]) = make_float2(l[0], l[1]);
+      uint32_t ph, pl;
+      split2(p[0], p[1], ph, pl);
+      *reinterpret_cast<uint32_t*>(item + 2 * kTri + tri_offset(i, c)) = ph;
+      *reinterpret_cast<uint32_t*>(item + 3 * kTri + tri_offset(i, c)) = pl;
+    }
+  }
+  float* vec = reinterpret_cast<float*>(item + 4 * kTri);
+  if (tid < kC) {
+    const float e = expf(s.bh[tid] + s.bl[tid]), last = s.bh[kC - 1], lastl = s.bl[kC - 1];
+    vec[tid] = s.beta[tid];
+    vec[kC + tid] = s.beta[tid] * e * s.rk[tid];
+    vec[2 * kC + tid] = expf((last - s.bh[tid]) + (lastl - s.bl[tid])) * s.rk[tid];
+    vec[3 * kC + tid] = e * s.rq[tid];
+    if (tid < 16) vec[4 * kC + tid] = tid == 0 ? expf(last + lastl) : 0.f;
+  }
+  __syncthreads();
+  // ---- X = (I + L)^-1 - I by forward substitution: thread j has column j ----
+  if (tid < kC) {
+    float x[kC];
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      float acc0 = 0.f, acc1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < i; k += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(&s.L[i][k]);
+        if (k < i) acc0 = fmaf(l.x, x[k], acc0);
+        if (k + 1 < i) acc1 = fmaf(l.y, x[k + 1], acc1);
+        if (k + 2 < i) acc0 = fmaf(l.z, x[k + 2], acc0);
+        if (k + 3 < i) acc1 = fmaf(l.w, x[k + 3], acc1);
+      }
+      const float lij = i > tid ? s.L[i][tid] : 0.f;
+      x[i] = i > tid ? -(acc0 + acc1) - lij : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+      if (i / 16 < tid / 16) continue;
+      const __nv_bfloat16 xh = __float2bfloat16(x[i]);
+      *reinterpret_cast<__nv_bfloat16*>(item + tri_offset(i, tid)) = xh;
+      *reinterpret_cast<__nv_bfloat16*>(item + kTri + tri_offset(i, tid)) = __float2bfloat16(x[i] - __bfloat162float(xh));
+    }
+  }
+  __syncthreads();
+  uint4* dst = reinterpret_cast<uint4*>(items + ((int64_t)w * a.HV + h) * kItemBytes);
+  for (int x = tid; x < kItemBytes / 16; x += 128) dst[x] = reinterpret_cast<const uint4*>(item)[x];
+}
+
+// ------------------------------------------------------------------------------------------------
+// The chain: one CTA per (request, value head). Everything is transposed, so that TMEM lanes are the 128 value columns
+// and the state never leaves the registers of the warps that own those lanes:
+//   warp 0       loader: k, q (128-byte swizzle), v tiles and the chunk's item, kStages ahead
+//   warp 1       TMEM owner; lane 0 issues the products
+//   warps 2-9    state warps: a thread has lane v and half of the 128 key columns of S (64 registers)
+//   warps 10-13  output warps: a thread has lane v and the chunk's 64 tokens
+// Per chunk (A operands in TMEM, B operands in shared memory, fp32 accumulators in TMEM):
+//   D1 = S^T k^T                          S pieces written by the state warps
+//   D2 = S^T q^T
+//   R  = beta v - c1 D1                   state warps; c1 = beta e^b / |k|
+//   D3 = R^T X^T, V' = R + D3             the identity part of (I + L)^-1 stays in fp32
+//   DS = (V' c2)^T k, S = e^(b_C) S + DS  c2 = e^(b_C - b) / |k|
+//   D4 = V'^T P^T, o = c3 D2 + D4         c3 = e^b scale / |q|
+// TMEM columns: S pieces 128 | D1, then R, then V' pieces 64 | D2, then D4 64 | D3, then V' c2 pieces 64 | DS 128.
+// A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
+// ------------------------------------------------------------------------------------------------
+constexpr int kStages = 3;
+constexpr int kChainThreads = 14 * 32;
+constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColDS = 320, kTmemCols = 512;
+constexpr int kStageTx = 3 * kC * kDim * 2 + kItemBytes;
+
+struct ChainStage {
+  uint8_t k[2][kC * 128];       // key dimensions 0-63 and 64-127, 128 bytes per token
+  uint8_t q[2][kC * 128];
+  __nv_bfloat16 v[kC][kDim];
+  uint8_t item[(kItemBytes + 1023) / 1024 * 1024];
+};
+struct ChainSmem {
+  ChainStage st[kStages];
+  uint64_t full[kStages], ready[kStages], empty[kStages];
+  uint64_t s_ready, r_ready, v_ready, d2_read, o_read;     // written by warps
+  uint64_t d1_full, d2_full, d3_full, ds_full, o_full;     // committed by the tensor core
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+};
+
+// MN-major SWIZZLE_128B operand: `lbo` bytes between 64-element blocks along N, 1024 between 8-row groups along K.
+__device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr, uint32_t lbo) {
+  return static_cast<uint64_t>((saddr & 0x3FFFF) >> 4) | static_cast<uint64_t>(lbo >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+// Unswizzled K-major operand: core matrices of 8 rows x 16 bytes, `lbo` bytes apart along K, 128 along N.
+__device__ __forceinline__ uint64_t sdesc_core(uint32_t saddr, uint32_t lbo) {
+  return static_cast<uint64_t>((saddr & 0x3FFFF) >> 4) | static_cast<uint64_t>(lbo >> 4) << 16 |
+         static_cast<uint64_t>(128 >> 4) << 32 | static_cast<uint64_t>(1) << 46;
+}
+
+// 1-D bulk copy of global memory into this CTA's shared memory, counted on `bar`
+__device__ __forceinline__ void bulk_load(uint64_t* bar, void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__global__ void __launch_bounds__(kChainThreads, 1)
+    gdn_chain_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ,
+                     const __grid_constant__ CUtensorMap tmV, const GdnArgs a, const uint8_t* __restrict__ items) {
+  extern __shared__ uint8_t smem_raw[];
+  ChainSmem& s = *reinterpret_cast<ChainSmem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
+  const int warp = warp_id(), lane = lane_id();
+  const int r = blockIdx.y, h = blockIdx.x, hk = h / (a.HV / a.HK);
+  int t0, t1, slot;
+  if (!request(a, r, t0, t1, slot) || t0 == t1) return;   // uniform, before any barrier or TMEM use
+  const int nchunks = (t1 - t0 + kC - 1) / kC;
+  const int tail = t1 - t0 - (nchunks - 1) * kC;           // tokens of the last chunk
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.ready[i], 1);
+      mbar_init(&s.empty[i], 5);       // the tensor core and the four output warps
+    }
+    for (uint64_t* b : {&s.s_ready, &s.r_ready, &s.v_ready}) mbar_init(b, 8);
+    for (uint64_t* b : {&s.d2_read, &s.o_read}) mbar_init(b, 4);
+    for (uint64_t* b : {&s.d1_full, &s.d2_full, &s.d3_full, &s.ds_full, &s.o_full, &s.mma_done}) mbar_init(b, 1);
+    s.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&s.tmem_base, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort = &s.abort;
+  int* status = a.status;
+
+  if (warp == 0) {
+    // ---------------- loader ----------------
+    const int item0 = first_item(a, r);
+    int issued = 0;
+    for (int c = 0; c < nchunks; ++c) {
+      const int st = c % kStages;
+      const uint32_t ph = (c / kStages) & 1;
+      ChainStage& g = s.st[st];
+      const bool ok = mbar_wait(&s.empty[st], ph ^ 1, status, kErrTimeoutProducer, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane == 0) {
+        const int t = t0 + c * kC;
+        mbar_arrive_expect_tx(&s.full[st], kStageTx);
+        tma_load_3d(&tmK, &s.full[st], g.k[0], 0, hk, t);
+        tma_load_3d(&tmK, &s.full[st], g.k[1], 64, hk, t);
+        bulk_load(&s.full[st], g.item, items + ((int64_t)(item0 + c) * a.HV + h) * kItemBytes, kItemBytes);
+        tma_load_3d(&tmQ, &s.full[st], g.q[0], 0, hk, t);
+        tma_load_3d(&tmQ, &s.full[st], g.q[1], 64, hk, t);
+        tma_load_3d(&tmV, &s.full[st], g.v, 0, h, t);
+      }
+      ++issued;
+      if (c == nchunks - 1 && tail < kC) {
+        // k rows past the request's end belong to another request: the update multiplies them by 0, so they have to
+        // be finite
+        const bool in = mbar_wait(&s.full[st], ph, status, kErrTimeoutProducer, abort);
+        if (!__all_sync(0xffffffffu, in)) break;
+        for (int x = lane; x < (kC - tail) * 16; x += 32)
+          *reinterpret_cast<uint4*>(&g.k[x & 1][(tail + (x >> 4)) * 128 + (x >> 1 & 7) * 16]) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(&s.ready[st]);
+    }
+    // the copies in flight land before the CTA may exit (bounded)
+    volatile int never = 0;
+    for (int c = max(0, issued - kStages); c < issued; ++c) mbar_wait(&s.full[c % kStages], (c / kStages) & 1, nullptr, 0, &never);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---------------- product issuer ----------------
+      constexpr uint32_t id64 = idesc_make(128, 64, 1), id128mn = idesc_make(128, 128, 1) | (1u << 16);
+      // D[128 x 64] = S^T B^T, B = k or q (K-major, key dimension 16 ks from column ks * 8 of each S piece)
+      auto state_product = [&](uint32_t d, const uint8_t (&b)[2][kC * 128]) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint64_t db = sdesc_sw128(smem_u32(b[ks >> 2])) + 2 * (ks & 3);
+          umma_f16_ts(tmem + d, tmem + kColS + ks * 8, db, id64, ks > 0);
+          umma_f16_ts(tmem + d, tmem + kColS + 64 + ks * 8, db, id64, 1);
+        }
+      };
+      // D[128 x 64] = A B^T, B lower triangular in two pieces; A in two pieces of 16 columns per 32 tokens
+      auto tri_product = [&](uint32_t d, uint32_t acol, const uint8_t* b) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const int rows = kC - 16 * ks;
+          const uint32_t id = idesc_make(128, rows, 1), base = smem_u32(b) + tri_start(ks);
+          const uint64_t hi = sdesc_core(base, rows * 16), lo = sdesc_core(base + kTri, rows * 16);
+          const uint32_t ahi = tmem + acol + (ks >> 1) * 32 + (ks & 1) * 8, alo = ahi + 16, dd = tmem + d + 16 * ks;
+          umma_f16_ts(dd, ahi, hi, id, ks > 0);
+          umma_f16_ts(dd, alo, hi, id, 1);
+          umma_f16_ts(dd, ahi, lo, id, 1);
+        }
+      };
+      for (int c = 0; c < nchunks; ++c) {
+        const int st = c % kStages;
+        const uint32_t ph = c & 1, sph = (c / kStages) & 1;
+        ChainStage& g = s.st[st];
+        if (!mbar_wait(&s.full[st], sph, status, kErrTimeoutMma, abort)) break;
+        if (!mbar_wait(&s.ready[st], sph, status, kErrTimeoutMma, abort)) break;
+        if (!mbar_wait(&s.s_ready, ph, status, kErrTimeoutMma, abort)) break;
+        tc_fence_after();
+        state_product(kColD1, g.k);
+        umma_commit(&s.d1_full);
+        if (c > 0 && !mbar_wait(&s.o_read, ph ^ 1, status, kErrTimeoutMma, abort)) break;
+        tc_fence_after();
+        state_product(kColD2, g.q);
+        umma_commit(&s.d2_full);
+        if (!mbar_wait(&s.r_ready, ph, status, kErrTimeoutMma, abort)) break;
+        tc_fence_after();
+        tri_product(kColD3, kColD1, g.item);
+        umma_commit(&s.d3_full);
+        if (!mbar_wait(&s.v_ready, ph, status, kErrTimeoutMma, abort)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const uint64_t db = sdesc_mn(smem_u32(g.k[0]) + ks * 2048, kC * 128);
+          const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
+          umma_f16_ts(tmem + kColDS, ahi, db, id128mn, ks > 0);
+          umma_f16_ts(tmem + kColDS, ahi + 16, db, id128mn, 1);
+        }
+        umma_commit(&s.ds_full);
+        if (!mbar_wait(&s.d2_read, ph, status, kErrTimeoutMma, abort)) break;
+        tc_fence_after();
+        tri_product(kColD2, kColD1, g.item + 2 * kTri);
+        umma_commit(&s.o_full);
+        umma_commit(&s.empty[st]);
+      }
+      umma_commit(&s.mma_done);
+      volatile int never = 0;
+      mbar_wait(&s.mma_done, 0, nullptr, 0, &never);
+    }
+  } else if (warp < 10) {
+    // ---------------- state warps ----------------
+    const int half = (warp - 2) >> 2, quad = warp & 3, v = quad * 32 + lane;
+    const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    float* gS = a.state + (((int64_t)slot * a.HV + h) * kDim + half * 64) * kDim + v;
+    float S[64];
+#pragma unroll
+    for (int j = 0; j < 64; ++j) S[j] = gS[j * kDim];
+    // 16 floats -> two bf16 pieces of 8 TMEM columns each
+    auto store_pieces = [&](uint32_t hi_col, uint32_t lo_col, const float* x) {
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
+      tmem_st8(tl + hi_col, hi);
+      tmem_st8(tl + lo_col, lo);
+    };
+    auto hand_over = [&](uint64_t* bar) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+      const bool ok = mbar_wait(bar, ph, status, kErrTimeoutEpilogue, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      return true;
+    };
+    bool ok = true;
+    for (int c = 0; c < nchunks; ++c) {
+      const int st = c % kStages, n = c == nchunks - 1 ? tail : kC;
+      const uint32_t ph = c & 1;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) store_pieces(kColS + half * 32 + g * 8, kColS + 64 + half * 32 + g * 8, S + 16 * g);
+      hand_over(&s.s_ready);
+
+      if (!(ok = wait(&s.full[st], (c / kStages) & 1))) break;
+      const float* vec = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + half * 32;
+      const float decay = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri)[4 * kC];
+      if (!(ok = wait(&s.d1_full, ph))) break;
+      float R[32];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t d[16];
+        tmem_ld16(tl + kColD1 + half * 32 + g * 16, d);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) R[16 * g + e] = __bfloat162float(s.st[st].v[half * 32 + 16 * g + e][v]) * vec[16 * g + e];
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = 16 * g + e;
+          R[i] = fmaf(-vec[kC + i], __uint_as_float(d[e]), R[i]);
+          if (half * 32 + i >= n) R[i] = 0.f;      // tokens past the request's end
+        }
+      }
+      // every column of this half is read before its pieces overwrite it
+#pragma unroll
+      for (int g = 0; g < 2; ++g) store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
+      hand_over(&s.r_ready);
+
+      if (!(ok = wait(&s.d3_full, ph))) break;
+      {
+        uint32_t d[32];
+        tmem_ld32(tl + kColD3 + half * 32, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) R[i] += __uint_as_float(d[i]);
+      }
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = R[16 * g + e] * vec[2 * kC + 16 * g + e];
+        store_pieces(kColD3 + half * 32 + g * 8, kColD3 + half * 32 + 16 + g * 8, x);
+        store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
+      }
+      hand_over(&s.v_ready);
+
+#pragma unroll
+      for (int j = 0; j < 64; ++j) S[j] *= decay;
+      if (!(ok = wait(&s.ds_full, ph))) break;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t d[32];
+        tmem_ld32(tl + kColDS + half * 64 + g * 32, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) S[32 * g + j] += __uint_as_float(d[j]);
+      }
+    }
+    if (ok) {
+#pragma unroll
+      for (int j = 0; j < 64; ++j) gS[j * kDim] = S[j];
+    }
+  } else {
+    // ---------------- output warps ----------------
+    const int quad = warp & 3, v = quad * 32 + lane;
+    const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+      const bool ok = mbar_wait(bar, ph, status, kErrTimeoutEpilogue, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      return true;
+    };
+    auto arrive = [&](uint64_t* bar) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    for (int c = 0; c < nchunks; ++c) {
+      const int st = c % kStages, n = c == nchunks - 1 ? tail : kC;
+      const uint32_t ph = c & 1;
+      float o[kC];
+      uint32_t d[32];
+      if (!wait(&s.full[st], (c / kStages) & 1)) break;
+      if (!wait(&s.d2_full, ph)) break;
+      const float* c3 = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + 3 * kC;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        tmem_ld32(tl + kColD2 + g * 32, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[32 * g + i] = __uint_as_float(d[i]) * c3[32 * g + i];
+      }
+      arrive(&s.d2_read);
+      if (!wait(&s.o_full, ph)) break;
+      __nv_bfloat16* out = a.out + ((int64_t)(t0 + c * kC) * a.HV + h) * kDim + v;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        tmem_ld32(tl + kColD2 + g * 32, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (32 * g + i < n) out[(int64_t)(32 * g + i) * a.HV * kDim] = __float2bfloat16(o[32 * g + i] + __uint_as_float(d[i]));
+      }
+      arrive(&s.o_read);
+      if (lane == 0) mbar_arrive(&s.empty[st]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
 }  // namespace
 
 void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g, torch::Tensor beta,
@@ -153,7 +698,38 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
             (int)T, (int)R, (int)HK, (int)HV, (int)state.size(0), (float)scale};
   const at::cuda::CUDAGuard guard(q.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  gdn_step_kernel<<<dim3((unsigned)R, (unsigned)HV), 256, 0, stream>>>(a);
+  auto rows16 = [](const torch::Tensor& t) {   // what 16-byte loads and tensor maps need
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+           t.stride(0) > 0 && t.stride(1) > 0;
+  };
+  if (T <= kStepMean * R || !rows16(q) || !rows16(k) || !rows16(v)) {
+    gdn_step_kernel<<<dim3((unsigned)R, (unsigned)HV), 256, 0, stream>>>(a);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    return;
+  }
+  TORCH_CHECK(R < 65536, "at most 65535 requests");
+  const int64_t n_items = T / kC + R;
+  torch::Tensor items = torch::empty({n_items * HV * kItemBytes}, q.options().dtype(at::kByte));
+  auto map = [&](const torch::Tensor& t, int64_t heads, uint32_t box, CUtensorMapSwizzle sw) {
+    return make_tmap_3d(t.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kDim, heads, T, t.stride(1) * 2, t.stride(0) * 2, box, 1,
+                        kC, sw);
+  };
+  const CUtensorMap tk = map(k, HK, 64, CU_TENSOR_MAP_SWIZZLE_128B), tq = map(q, HK, 64, CU_TENSOR_MAP_SWIZZLE_128B),
+                    tv = map(v, HV, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static bool opted[64] = {};   // the opt-in belongs to each device's context
+  TORCH_CHECK(dev < 64, "device index out of range");
+  constexpr int chain_smem = sizeof(ChainSmem) + 1024, prep_smem = sizeof(PrepSmem);
+  if (!opted[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(gdn_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, chain_smem));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(gdn_prep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, prep_smem));
+    opted[dev] = true;
+  }
+  uint8_t* it = items.data_ptr<uint8_t>();
+  gdn_prep_kernel<<<dim3((unsigned)n_items, (unsigned)HV), 128, prep_smem, stream>>>(a, it);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  gdn_chain_kernel<<<dim3((unsigned)HV, (unsigned)R), kChainThreads, chain_smem, stream>>>(tk, tq, tv, a, it);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

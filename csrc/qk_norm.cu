@@ -95,6 +95,95 @@ __global__ void __launch_bounds__(256) qk_norm_rope_narrow_kernel(const QkArgs a
   }
 }
 
+// Aligned rows and D = 8 L for L = 8, 16 or 32 lanes: a lane holds two runs of four elements of a head that are each
+// other's rotation partners (elements 4 i and rot / 2 + 4 i; in the part that is not rotated, any two runs), so the
+// rotation needs no exchange and a lane four (cos, sin) pairs and eight weights, which it loads once. A warp takes 32 / L
+// heads of one token at a time and P such groups in all, whose loads are issued together.
+template <int L, int P>
+__global__ void __launch_bounds__(256) qk_norm_rope_wide_kernel(const QkArgs a) {
+  constexpr int kHeads = 32 / L, D = 8 * L;
+  const int nh = a.Hq + 2 * a.Hkv;
+  const int groups = (nh + kHeads * P - 1) / (kHeads * P);
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= (int64_t)a.M * groups) return;
+  const int t = (int)(w / groups), h0 = (int)(w - (int64_t)t * groups) * kHeads * P;
+  const int lane = threadIdx.x & 31, i = lane % L, sub = lane / L;
+  const bool turned = i < (a.rot >> 3);
+  const int e1 = turned ? 4 * i : a.rot + 4 * (i - (a.rot >> 3));
+  const int e2 = e1 + (turned ? a.rot >> 1 : (D - a.rot) >> 1);
+  const __nv_bfloat16* src = a.qkv + (int64_t)t * a.ld + (int64_t)(h0 + sub) * D;
+  uint2 x1[P], x2[P];
+#pragma unroll
+  for (int u = 0; u < P; ++u) {
+    x1[u] = x2[u] = make_uint2(0, 0);
+    if (h0 + u * kHeads + sub < nh) {
+      x1[u] = *reinterpret_cast<const uint2*>(src + u * kHeads * D + e1);
+      x2[u] = *reinterpret_cast<const uint2*>(src + u * kHeads * D + e2);
+    }
+  }
+  float2 cs[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) cs[e] = make_float2(1.f, 0.f);
+  if (turned) {
+    const float4* c4 = reinterpret_cast<const float4*>(a.cos_sin + (int64_t)table_row(a, t) * (a.rot >> 1) + 4 * i);
+    const float4 lo = c4[0], hi = c4[1];
+    cs[0] = make_float2(lo.x, lo.y), cs[1] = make_float2(lo.z, lo.w);
+    cs[2] = make_float2(hi.x, hi.y), cs[3] = make_float2(hi.z, hi.w);
+  }
+  const uint2 q1 = *reinterpret_cast<const uint2*>(a.wq + e1), q2 = *reinterpret_cast<const uint2*>(a.wq + e2);
+  const uint2 k1 = *reinterpret_cast<const uint2*>(a.wk + e1), k2 = *reinterpret_cast<const uint2*>(a.wk + e2);
+  const int64_t base = h0 + kHeads * P > a.Hq ? cache_base(a, t) : -1;
+#pragma unroll
+  for (int u = 0; u < P; ++u) {
+    const int h = h0 + u * kHeads + sub;
+    const float2 a0 = unpack_bf16x2(x1[u].x), a1 = unpack_bf16x2(x1[u].y), b0 = unpack_bf16x2(x2[u].x), b1 = unpack_bf16x2(x2[u].y);
+    float ss = fmaf(a0.x, a0.x, a0.y * a0.y) + fmaf(a1.x, a1.x, a1.y * a1.y) +
+               (fmaf(b0.x, b0.x, b0.y * b0.y) + fmaf(b1.x, b1.x, b1.y * b1.y));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (h >= nh) continue;
+    uint2 r1 = x1[u], r2 = x2[u];
+    if (h < a.Hq + a.Hkv) {
+      const float inv = rsqrtf(ss / D + a.eps);
+      const bool is_q = h < a.Hq;
+      const float2 g0 = unpack_bf16x2(is_q ? q1.x : k1.x), g1 = unpack_bf16x2(is_q ? q1.y : k1.y);
+      const float2 f0 = unpack_bf16x2(is_q ? q2.x : k2.x), f1 = unpack_bf16x2(is_q ? q2.y : k2.y);
+      const float y[4] = {a0.x * inv * g0.x, a0.y * inv * g0.y, a1.x * inv * g1.x, a1.y * inv * g1.y};
+      const float z[4] = {b0.x * inv * f0.x, b0.y * inv * f0.y, b1.x * inv * f1.x, b1.y * inv * f1.y};
+      float o1[4], o2[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {        // an infinity in one part of the other run stays out of what is not rotated
+        o1[e] = turned ? y[e] * cs[e].x - z[e] * cs[e].y : y[e];
+        o2[e] = turned ? z[e] * cs[e].x + y[e] * cs[e].y : z[e];
+      }
+      r1 = make_uint2(pack_bf16x2(o1[0], o1[1]), pack_bf16x2(o1[2], o1[3]));
+      r2 = make_uint2(pack_bf16x2(o2[0], o2[1]), pack_bf16x2(o2[2], o2[3]));
+    }
+    __nv_bfloat16* dst;
+    if (h < a.Hq) {
+      dst = a.q_out + ((int64_t)t * a.Hq + h) * D;
+    } else {
+      if (base < 0) continue;
+      const bool is_k = h < a.Hq + a.Hkv;
+      dst = (is_k ? a.k_cache : a.v_cache) + base + (int64_t)(h - a.Hq - (is_k ? 0 : a.Hkv)) * a.page_size * D;
+    }
+    *reinterpret_cast<uint2*>(dst + e1) = r1;
+    *reinterpret_cast<uint2*>(dst + e2) = r2;
+  }
+}
+
+template <int L>
+void launch_wide(const QkArgs& a, cudaStream_t stream) {
+  constexpr int kHeads = 32 / L;
+  const int nh = a.Hq + 2 * a.Hkv;
+  // Groups per warp: 8 share the cos/sin and weight loads, 1 spreads a small batch over more SMs.
+  const auto warps = [&](int p) { return (int64_t)a.M * ((nh + kHeads * p - 1) / (kHeads * p)); };
+  if (warps(8) >= 148 * 32)
+    qk_norm_rope_wide_kernel<L, 8><<<(unsigned)((warps(8) + 7) / 8), 256, 0, stream>>>(a);
+  else
+    qk_norm_rope_wide_kernel<L, 1><<<(unsigned)((warps(1) + 7) / 8), 256, 0, stream>>>(a);
+}
+
 }  // namespace
 
 void qk_norm_rope_kv_write(torch::Tensor qkv, torch::Tensor wq, torch::Tensor wk, double eps, torch::Tensor pos,
@@ -149,8 +238,16 @@ void qk_norm_rope_kv_write(torch::Tensor qkv, torch::Tensor wq, torch::Tensor wk
   a.eps = (float)eps;
   const at::cuda::CUDAGuard guard(qkv.device());
   auto stream = at::cuda::getCurrentCUDAStream();
+  auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool wide = a.rot % 8 == 0 && a.ld % 8 == 0 && aligned(a.qkv) && aligned(a.wq) && aligned(a.wk) &&
+                    aligned(a.cos_sin) && aligned(a.q_out) && aligned(a.k_cache) && aligned(a.v_cache);
+  if (wide && D == 64) launch_wide<8>(a, stream);
+  else if (wide && D == 128) launch_wide<16>(a, stream);
+  else if (wide && D == 256) launch_wide<32>(a, stream);
+  else {
   const int64_t warps = M * (Hq + 2 * Hkv);
   qk_norm_rope_narrow_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, stream>>>(a);
+  }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
