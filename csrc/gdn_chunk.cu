@@ -17,6 +17,7 @@ namespace phx {
 namespace {
 
 constexpr int kDim = 128;
+constexpr double kLog2e = 1.4426950408889634;
 
 struct GdnArgs {
   const __nv_bfloat16 *q, *k, *v;
@@ -170,26 +171,62 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// D += A B in fp32 to about 2^-21: each operand as two tf32 parts, the product of the two small ones left out
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma_split(float (&d)[4], const float (&a)[4], const float (&b)[2]) {
+  uint32_t ah[4], al[4], bh[2], bl[2];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    ah[e] = __float_as_uint(a[e]) & 0xffffe000u;
+    al[e] = __float_as_uint(a[e] - __uint_as_float(ah[e]));
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    bh[e] = __float_as_uint(b[e]) & 0xffffe000u;
+    bl[e] = __float_as_uint(b[e] - __uint_as_float(bh[e]));
+  }
+  mma_tf32(d, al, bh);
+  mma_tf32(d, ah, bl);
+  mma_tf32(d, ah, bh);
+}
+
 constexpr int kPrepRow = kDim + 8;     // bf16 elements of a padded shared row: ldmatrix's eight rows miss each other's banks
-constexpr int kLRow = kC + 4;
+constexpr int kBlkRow = 20;            // floats of a padded row of a 16 x 16 block
+constexpr int kWRow = 12;
 struct PrepSmem {
   union {
     struct {
       __nv_bfloat16 k[kC][kPrepRow], q[kC][kPrepRow];
     } in;
-    uint8_t item[kItemBytes];          // the finished item, copied out in one go
+    struct {
+      float blk[10][16][kBlkRow];      // the blocks on and below the diagonal: L, then (I + L)^-1 in its place
+      float w[4][32][kWRow];           // each warp's 8 columns of a product
+    } inv;
   };
-  float L[kC][kLRow];
-  float bh[kC], bl[kC];                // b as the sum of two floats: differences of far-down sums keep their digits
+  float bh[kC], bl[kC];                // b / ln 2 as the sum of two floats: differences of far-down sums keep their digits
   float rk[kC], rq[kC], beta[kC];
 };
+__host__ __device__ constexpr int blk_of(int bi, int bj) { return bi * (bi + 1) / 2 + bj; }
 
-// One CTA per (work item, value head).
-__global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t* __restrict__ items) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  PrepSmem& s = *reinterpret_cast<PrepSmem*>(smem_raw);
-  const int w = blockIdx.x, h = blockIdx.y, hk = h / (a.HV / a.HK);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// One CTA per (work item, `heads` value heads of one key head). The Gram matrices come from mma.sync and stay in its
+// registers; each head's P and factors go from there to memory (a warp's 4-byte stores fill 128 bytes). (I + L)^-1 by
+// blocks of 16: the diagonal ones by forward substitution, one column per thread, then 16 -> 32 -> 64 by
+// T_BA = -T_BB (L_BA T_AA). Each entry is a true entry of the inverse on the way (no powers of L, which can grow where
+// keys repeat).
+__global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8_t* __restrict__ items, int heads) {
+  __shared__ __align__(128) PrepSmem s;
+  const int w = blockIdx.x, hk = blockIdx.y * heads / (a.HV / a.HK);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int lo = 0, hi = a.R - 1;            // the last request whose items start at or before w
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -197,14 +234,15 @@ __global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t*
     else hi = mid - 1;
   }
   int t0, t1, slot;
-  if (!request(a, lo, t0, t1, slot)) return;
+  if (!request(a, lo, t0, t1, slot) || w < first_item(a, lo)) return;
   t0 += (w - first_item(a, lo)) * kC;
   const int n = min(kC, t1 - t0);
-  if (n <= 0 || w < first_item(a, lo)) return;
+  if (n <= 0) return;
 
-  // ---- q and k rows (zeros past the request's end), factors ----
-  for (int x = tid; x < kC * 16; x += 128) {
-    const int row = x >> 4, c = (x & 15) * 8;
+  // ---- q and k rows (zeros past the request's end) ----
+#pragma unroll
+  for (int x0 = 0; x0 < kC * 16; x0 += 128) {
+    const int row = (x0 + tid) >> 4, c = (tid & 15) * 8;
     uint4 kv = make_uint4(0, 0, 0, 0), qv = kv;
     if (row < n) {
       kv = *reinterpret_cast<const uint4*>(a.k + (int64_t)(t0 + row) * a.k_t + hk * a.k_h + c);
@@ -213,27 +251,11 @@ __global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t*
     *reinterpret_cast<uint4*>(&s.in.k[row][c]) = kv;
     *reinterpret_cast<uint4*>(&s.in.q[row][c]) = qv;
   }
-  if (warp == 0) {
-    double b0 = 2 * lane < n ? a.g[(int64_t)(t0 + 2 * lane) * a.HV + h] : 0.f;
-    double b1 = b0 + (2 * lane + 1 < n ? a.g[(int64_t)(t0 + 2 * lane + 1) * a.HV + h] : 0.f);
-    double inc = b1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    b0 += inc - b1;
-    s.bh[2 * lane] = (float)b0, s.bl[2 * lane] = (float)(b0 - (float)b0);
-    s.bh[2 * lane + 1] = (float)inc, s.bl[2 * lane + 1] = (float)(inc - (float)inc);
-  } else if (warp < 3) {
-    const int i = tid - 32;
-    s.beta[i] = i < n ? a.beta[(int64_t)(t0 + i) * a.HV + h] : 0.f;
-  }
   __syncthreads();
   {
     const int row = tid & 63;
     const uint4* src = reinterpret_cast<const uint4*>(tid < 64 ? s.in.k[row] : s.in.q[row]);
-    float ss = 0.f;
+    float ss = 0.f, s2 = 0.f;
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
       const uint4 u = src[c];
@@ -241,10 +263,11 @@ __global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t*
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 f = unpack_bf16x2(x[e]);
-        ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+        ss = fmaf(f.x, f.x, ss);
+        s2 = fmaf(f.y, f.y, s2);
       }
     }
-    (tid < 64 ? s.rk : s.rq)[row] = rsqrtf(ss + 1e-6f) * (tid < 64 ? 1.f : a.scale);
+    (tid < 64 ? s.rk : s.rq)[row] = rsqrtf(ss + s2 + 1e-6f) * (tid < 64 ? 1.f : a.scale);
   }
 
   // ---- Gram matrices k k^T and q k^T: warp w has rows 16 w .. 16 w + 15, columns up to the diagonal block ----
@@ -261,83 +284,200 @@ __global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t*
     ldmatrix_x4(aq, smem_u32(&s.in.q[ar][ac]));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {        // two column tiles of 8 at a time
-      if (j > warp) break;
-      uint32_t b[4];
-      ldmatrix_x4(b, smem_u32(&s.in.k[j * 16 + (lane >> 4) * 8 + (lane & 7)][ks * 16 + (lane >> 3 & 1) * 8]));
-      mma_bf16(kk[2 * j], ak, b[0], b[1]);
-      mma_bf16(kk[2 * j + 1], ak, b[2], b[3]);
-      mma_bf16(qk[2 * j], aq, b[0], b[1]);
-      mma_bf16(qk[2 * j + 1], aq, b[2], b[3]);
+      if (j <= warp) {
+        uint32_t b[4];
+        ldmatrix_x4(b, smem_u32(&s.in.k[j * 16 + (lane >> 4) * 8 + (lane & 7)][ks * 16 + (lane >> 3 & 1) * 8]));
+        mma_bf16(kk[2 * j], ak, b[0], b[1]);
+        mma_bf16(kk[2 * j + 1], ak, b[2], b[3]);
+        mma_bf16(qk[2 * j], aq, b[0], b[1]);
+        mma_bf16(qk[2 * j + 1], aq, b[2], b[3]);
+      }
     }
   }
-  __syncthreads();     // the item's bytes take the place of k and q; the factors are complete
-  uint8_t* item = s.item;
+
+  for (int hh = 0; hh < heads; ++hh) {
+    const int h = blockIdx.y * heads + hh;
+    uint8_t* item = items + ((int64_t)w * a.HV + h) * kItemBytes;
+    // ---- the head's sums of g and betas ----
+    if (warp == 0) {
+      // e^-1e6 is 0 as e^-inf is, and its sums can be subtracted
+      auto gate = [&](int i) -> double {
+        const float x = i < n ? a.g[(int64_t)(t0 + i) * a.HV + h] : 0.f;
+        return x < -1e6f ? -1e6f : x;
+      };
+      double b0 = gate(2 * lane);
+      const double b1 = b0 + gate(2 * lane + 1);
+      double inc = b1;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (j > 2 * warp + 1) break;
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      b0 += inc - b1;
+      b0 *= kLog2e;
+      inc *= kLog2e;
+      s.bh[2 * lane] = (float)b0, s.bl[2 * lane] = (float)(b0 - (float)b0);
+      s.bh[2 * lane + 1] = (float)inc, s.bl[2 * lane + 1] = (float)(inc - (float)inc);
+    } else if (warp < 3) {
+      const int i = tid - 32;
+      s.beta[i] = i < n ? a.beta[(int64_t)(t0 + i) * a.HV + h] : 0.f;
+    }
+    __syncthreads();     // the blocks take the place of k and q (or of the last head's blocks); the factors are complete
+    float* vec = reinterpret_cast<float*>(item + 4 * kTri);
+    if (tid < kC) {
+      const float e = exp2_approx(s.bh[tid] + s.bl[tid]), last = s.bh[kC - 1], lastl = s.bl[kC - 1];
+      vec[tid] = s.beta[tid];
+      vec[kC + tid] = s.beta[tid] * e * s.rk[tid];
+      vec[2 * kC + tid] = exp2_approx((last - s.bh[tid]) + (lastl - s.bl[tid])) * s.rk[tid];
+      vec[3 * kC + tid] = e * s.rq[tid];
+      if (tid < 16) vec[4 * kC + tid] = tid == 0 ? exp2_approx(last + lastl) : 0.f;
+    }
 #pragma unroll
     for (int e2 = 0; e2 < 2; ++e2) {
-      const int i = warp * 16 + (lane >> 2) + 8 * e2, c = j * 8 + (lane & 3) * 2;
-      float l[2], p[2];
+      const int i = warp * 16 + g + 8 * e2;
+      const float bhi = s.bh[i], bli = s.bl[i], fk = s.beta[i] * s.rk[i], fq = s.rq[i];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float d = c + e <= i ? expf((s.bh[i] - s.bh[c + e]) + (s.bl[i] - s.bl[c + e])) * s.rk[c + e] : 0.f;
-        l[e] = c + e < i ? kk[j][2 * e2 + e] * d * (s.beta[i] * s.rk[i]) : 0.f;
-        p[e] = c + e <= i ? qk[j][2 * e2 + e] * d * s.rq[i] : 0.f;
+      for (int j = 0; j < 8; ++j) {
+        if (j <= 2 * warp + 1) {
+          const int c = j * 8 + t * 2;
+          const float2 ch = *reinterpret_cast<const float2*>(&s.bh[c]), cl = *reinterpret_cast<const float2*>(&s.bl[c]);
+          const float2 cr = *reinterpret_cast<const float2*>(&s.rk[c]);
+          const float d0 = c <= i ? exp2_approx((bhi - ch.x) + (bli - cl.x)) * cr.x : 0.f;
+          const float d1 = c < i ? exp2_approx((bhi - ch.y) + (bli - cl.y)) * cr.y : 0.f;
+          const float l0 = c < i ? kk[j][2 * e2] * d0 * fk : 0.f, l1 = c + 1 < i ? kk[j][2 * e2 + 1] * d1 * fk : 0.f;
+          *reinterpret_cast<float2*>(&s.inv.blk[blk_of(warp, j >> 1)][i & 15][c & 15]) = make_float2(l0, l1);
+          uint32_t ph, pl;
+          split2(qk[j][2 * e2] * d0 * fq, qk[j][2 * e2 + 1] * d1 * fq, ph, pl);
+          *reinterpret_cast<uint32_t*>(item + 2 * kTri + tri_offset(i, c)) = ph;
+          *reinterpret_cast<uint32_t*>(item + 3 * kTri + tri_offset(i, c)) = pl;
+        }
       }
-      *reinterpret_cast<float2*>(&s.L[i][c]) = make_float2(l[0], l[1]);
-      uint32_t ph, pl;
-      split2(p[0], p[1], ph, pl);
-      *reinterpret_cast<uint32_t*>(item + 2 * kTri + tri_offset(i, c)) = ph;
-      *reinterpret_cast<uint32_t*>(item + 3 * kTri + tri_offset(i, c)) = pl;
     }
-  }
-  float* vec = reinterpret_cast<float*>(item + 4 * kTri);
-  if (tid < kC) {
-    const float e = expf(s.bh[tid] + s.bl[tid]), last = s.bh[kC - 1], lastl = s.bl[kC - 1];
-    vec[tid] = s.beta[tid];
-    vec[kC + tid] = s.beta[tid] * e * s.rk[tid];
-    vec[2 * kC + tid] = expf((last - s.bh[tid]) + (lastl - s.bl[tid])) * s.rk[tid];
-    vec[3 * kC + tid] = e * s.rq[tid];
-    if (tid < 16) vec[4 * kC + tid] = tid == 0 ? expf(last + lastl) : 0.f;
-  }
-  __syncthreads();
-  // ---- X = (I + L)^-1 - I by forward substitution: thread j has column j ----
-  if (tid < kC) {
-    float x[kC];
+    __syncwarp();
+    // ---- diagonal blocks: warp w has block w, lane j < 16 column j ----
+    float (*D)[kBlkRow] = s.inv.blk[blk_of(warp, warp)];
+    {
+      float x[16];
+      const int col = lane & 15;
 #pragma unroll
-    for (int i = 0; i < kC; ++i) {
-      float acc0 = 0.f, acc1 = 0.f;
+      for (int i = 0; i < 16; ++i) {
+        float l[16];
 #pragma unroll
-      for (int k = 0; k < i; k += 4) {
-        const float4 l = *reinterpret_cast<const float4*>(&s.L[i][k]);
-        if (k < i) acc0 = fmaf(l.x, x[k], acc0);
-        if (k + 1 < i) acc1 = fmaf(l.y, x[k + 1], acc1);
-        if (k + 2 < i) acc0 = fmaf(l.z, x[k + 2], acc0);
-        if (k + 3 < i) acc1 = fmaf(l.w, x[k + 3], acc1);
+        for (int k = 0; k < i; k += 4) *reinterpret_cast<float4*>(&l[k]) = *reinterpret_cast<const float4*>(&D[i][k]);
+        float a0 = i == col ? 1.f : 0.f, a1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < i; k += 2) {
+          a0 = fmaf(-l[k], x[k], a0);
+          if (k + 1 < i) a1 = fmaf(-l[k + 1], x[k + 1], a1);
+        }
+        x[i] = a0 + a1;
       }
-      const float lij = i > tid ? s.L[i][tid] : 0.f;
-      x[i] = i > tid ? -(acc0 + acc1) - lij : 0.f;
-    }
+      __syncwarp();
+      if (lane < 16) {
 #pragma unroll
-    for (int i = 0; i < kC; ++i) {
-      if (i / 16 < tid / 16) continue;
-      const __nv_bfloat16 xh = __float2bfloat16(x[i]);
-      *reinterpret_cast<__nv_bfloat16*>(item + tri_offset(i, tid)) = xh;
-      *reinterpret_cast<__nv_bfloat16*>(item + kTri + tri_offset(i, tid)) = __float2bfloat16(x[i] - __bfloat162float(xh));
+        for (int i = 0; i < 16; ++i) D[i][col] = x[i];
+      }
     }
+    __syncthreads();
+    float (*W)[kWRow] = s.inv.w[warp];
+    auto load_a = [&](float (&f)[4], const float (*b)[kBlkRow], int k0) {
+      f[0] = b[g][k0 + t], f[1] = b[g + 8][k0 + t], f[2] = b[g][k0 + t + 4], f[3] = b[g + 8][k0 + t + 4];
+    };
+    // ---- 16 -> 32: warp w has pair w / 2 and columns 8 (w % 2) .. of its block ----
+    {
+      const int lo_b = (warp >> 1) * 2, c0 = (warp & 1) * 8;
+      float (*BA)[kBlkRow] = s.inv.blk[blk_of(lo_b + 1, lo_b)];
+      const float (*AA)[kBlkRow] = s.inv.blk[blk_of(lo_b, lo_b)], (*BB)[kBlkRow] = s.inv.blk[blk_of(lo_b + 1, lo_b + 1)];
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k0 = 0; k0 < 16; k0 += 8) {
+        float fa[4], fb[2] = {AA[k0 + t][c0 + g], AA[k0 + t + 4][c0 + g]};
+        load_a(fa, BA, k0);
+        mma_split(d, fa, fb);
+      }
+      W[g][2 * t] = d[0], W[g][2 * t + 1] = d[1], W[g + 8][2 * t] = d[2], W[g + 8][2 * t + 1] = d[3];
+      __syncthreads();            // both halves of the pair have read L_BA
+      float r[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k0 = 0; k0 < 16; k0 += 8) {
+        float fa[4], fb[2] = {W[k0 + t][g], W[k0 + t + 4][g]};
+        load_a(fa, BB, k0);
+        mma_split(r, fa, fb);
+      }
+      BA[g][c0 + 2 * t] = -r[0], BA[g][c0 + 2 * t + 1] = -r[1], BA[g + 8][c0 + 2 * t] = -r[2], BA[g + 8][c0 + 2 * t + 1] = -r[3];
+    }
+    __syncthreads();
+    // ---- 32 -> 64: warp w has columns 8 w .. 8 w + 7 ----
+    {
+      const int bc = warp >> 1, c0 = (warp & 1) * 8;
+      float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int bk = 0; bk < 2; ++bk) {          // T_AA: block (0, 1) is zero
+        if (bk < bc) continue;
+        const float (*AA)[kBlkRow] = s.inv.blk[blk_of(bk, bc)];
+#pragma unroll
+        for (int k0 = 0; k0 < 16; k0 += 8) {
+          const float fb[2] = {AA[k0 + t][c0 + g], AA[k0 + t + 4][c0 + g]};
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            float fa[4];
+            load_a(fa, s.inv.blk[blk_of(2 + m, bk)], k0);
+            mma_split(d[m], fa, fb);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        W[16 * m + g][2 * t] = d[m][0], W[16 * m + g][2 * t + 1] = d[m][1], W[16 * m + g + 8][2 * t] = d[m][2], W[16 * m + g + 8][2 * t + 1] = d[m][3];
+      __syncthreads();            // every warp has read L_BA
+      float r[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int bk = 0; bk < 2; ++bk)
+#pragma unroll
+        for (int k0 = 0; k0 < 16; k0 += 8) {
+          const float fb[2] = {W[16 * bk + k0 + t][g], W[16 * bk + k0 + t + 4][g]};
+#pragma unroll
+          for (int m = bk; m < 2; ++m) {        // T_BB: block (2, 3) is zero
+            float fa[4];
+            load_a(fa, s.inv.blk[blk_of(2 + m, 2 + bk)], k0);
+            mma_split(r[m], fa, fb);
+          }
+        }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float (*BA)[kBlkRow] = s.inv.blk[blk_of(2 + m, bc)];
+        BA[g][c0 + 2 * t] = -r[m][0], BA[g][c0 + 2 * t + 1] = -r[m][1];
+        BA[g + 8][c0 + 2 * t] = -r[m][2], BA[g + 8][c0 + 2 * t + 1] = -r[m][3];
+      }
+    }
+    __syncthreads();
+    // ---- X pieces: eight neighbouring columns of a row at a time ----
+    for (int x = tid; x < 320; x += 128) {
+      const int bi_bj = x >> 5, row = x & 15, c = (x >> 4 & 1) * 8;
+      const int bi = bi_bj < 1 ? 0 : bi_bj < 3 ? 1 : bi_bj < 6 ? 2 : 3, bj = bi_bj - bi * (bi + 1) / 2;
+      float f[8];
+      *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(&s.inv.blk[bi_bj][row][c]);
+      *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(&s.inv.blk[bi_bj][row][c + 4]);
+      uint32_t xh[4], xl[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (bi == bj && c + e == row) f[e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split2(f[2 * e], f[2 * e + 1], xh[e], xl[e]);
+      const int at = tri_offset(bi * 16 + row, bj * 16 + c);
+      *reinterpret_cast<uint4*>(item + at) = make_uint4(xh[0], xh[1], xh[2], xh[3]);
+      *reinterpret_cast<uint4*>(item + kTri + at) = make_uint4(xl[0], xl[1], xl[2], xl[3]);
+    }
+    __syncthreads();     // the next head rewrites the blocks
   }
-  __syncthreads();
-  uint4* dst = reinterpret_cast<uint4*>(items + ((int64_t)w * a.HV + h) * kItemBytes);
-  for (int x = tid; x < kItemBytes / 16; x += 128) dst[x] = reinterpret_cast<const uint4*>(item)[x];
 }
 
 // ------------------------------------------------------------------------------------------------
 // The chain: one CTA per (request, value head). Everything is transposed, so that TMEM lanes are the 128 value columns
 // and the state never leaves the registers of the warps that own those lanes:
 //   warp 0       loader: k, q (128-byte swizzle), v tiles and the chunk's item, kStages ahead
-//   warp 1       TMEM owner; lane 0 issues the products
-//   warps 2-9    state warps: a thread has lane v and half of the 128 key columns of S (64 registers)
+//   warp 1       TMEM owner; issues the products
+//   warps 2-9    state warps: a thread has lane v and the key columns g * 64 + half * 32 + 0..31, g = 0, 1, of S
 //   warps 10-13  output warps: a thread has lane v and the chunk's 64 tokens
 // Per chunk (A operands in TMEM, B operands in shared memory, fp32 accumulators in TMEM):
 //   D1 = S^T k^T                          S pieces written by the state warps
@@ -346,6 +486,8 @@ __global__ void __launch_bounds__(128) gdn_prep_kernel(const GdnArgs a, uint8_t*
 //   D3 = R^T X^T, V' = R + D3             the identity part of (I + L)^-1 stays in fp32
 //   DS = (V' c2)^T k, S = e^(b_C) S + DS  c2 = e^(b_C - b) / |k|
 //   D4 = V'^T P^T, o = c3 D2 + D4         c3 = e^b scale / |q|
+// The chain's latency bounds it: S -> D1 -> R -> D3 -> V' -> DS -> S. S goes through in two halves of 64 key columns, so
+// that converting one overlaps the products of the other; D2 and D4 fill the tensor core's gaps.
 // TMEM columns: S pieces 128 | D1, then R, then V' pieces 64 | D2, then D4 64 | D3, then V' c2 pieces 64 | DS 128.
 // A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
 // ------------------------------------------------------------------------------------------------
@@ -363,8 +505,8 @@ struct ChainStage {
 struct ChainSmem {
   ChainStage st[kStages];
   uint64_t full[kStages], ready[kStages], empty[kStages];
-  uint64_t s_ready, r_ready, v_ready, d2_read, o_read;     // written by warps
-  uint64_t d1_full, d2_full, d3_full, ds_full, o_full;     // committed by the tensor core
+  uint64_t s_ready[2], r_ready, v_ready, p_ready, d2_read, o_read, o_staged;     // written by warps
+  uint64_t d1_full, d2_full, d3_full, ds_full[2], o_full;                        // committed by the tensor core
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
@@ -406,9 +548,9 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       mbar_init(&s.ready[i], 1);
       mbar_init(&s.empty[i], 5);       // the tensor core and the four output warps
     }
-    for (uint64_t* b : {&s.s_ready, &s.r_ready, &s.v_ready}) mbar_init(b, 8);
-    for (uint64_t* b : {&s.d2_read, &s.o_read}) mbar_init(b, 4);
-    for (uint64_t* b : {&s.d1_full, &s.d2_full, &s.d3_full, &s.ds_full, &s.o_full, &s.mma_done}) mbar_init(b, 1);
+    for (uint64_t* b : {&s.s_ready[0], &s.s_ready[1], &s.r_ready, &s.v_ready, &s.p_ready}) mbar_init(b, 8);
+    for (uint64_t* b : {&s.d2_read, &s.o_read, &s.o_staged}) mbar_init(b, 4);
+    for (uint64_t* b : {&s.d1_full, &s.d2_full, &s.d3_full, &s.ds_full[0], &s.ds_full[1], &s.o_full, &s.mma_done}) mbar_init(b, 1);
     s.abort = 0;
     fence_mbar_init();
   }
@@ -460,77 +602,86 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     volatile int never = 0;
     for (int c = max(0, issued - kStages); c < issued; ++c) mbar_wait(&s.full[c % kStages], (c / kStages) & 1, nullptr, 0, &never);
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---------------- product issuer ----------------
-      constexpr uint32_t id64 = idesc_make(128, 64, 1), id128mn = idesc_make(128, 128, 1) | (1u << 16);
-      // D[128 x 64] = S^T B^T, B = k or q (K-major, key dimension 16 ks from column ks * 8 of each S piece)
-      auto state_product = [&](uint32_t d, const uint8_t (&b)[2][kC * 128]) {
+    // ---------------- product issuer: the whole warp walks the loop, one elected lane issues. (A branch for one lane
+    // around the loop keeps descriptors out of the uniform registers: 78 instead of 32 cycles a 64-column product.)
+    constexpr uint32_t id64 = idesc_make(128, 64, 1), id64mn = id64 | (1u << 16);
+    auto wait = [&](uint64_t* bar, uint32_t ph) {
+      const bool ok = mbar_wait(bar, ph, status, kErrTimeoutMma, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      return true;
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) umma_commit(bar);
+    };
+    // D[128 x 64] += S^T B^T over key dimensions 64 g .. 64 g + 63, B = k or q (K-major)
+    auto state_product = [&](uint32_t d, const uint8_t* b, int g) {
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint64_t db = sdesc_sw128(smem_u32(b[ks >> 2])) + 2 * (ks & 3);
-          umma_f16_ts(tmem + d, tmem + kColS + ks * 8, db, id64, ks > 0);
-          umma_f16_ts(tmem + d, tmem + kColS + 64 + ks * 8, db, id64, 1);
-        }
-      };
-      // D[128 x 64] = A B^T, B lower triangular in two pieces; A in two pieces of 16 columns per 32 tokens
-      auto tri_product = [&](uint32_t d, uint32_t acol, const uint8_t* b) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const int rows = kC - 16 * ks;
-          const uint32_t id = idesc_make(128, rows, 1), base = smem_u32(b) + tri_start(ks);
-          const uint64_t hi = sdesc_core(base, rows * 16), lo = sdesc_core(base + kTri, rows * 16);
-          const uint32_t ahi = tmem + acol + (ks >> 1) * 32 + (ks & 1) * 8, alo = ahi + 16, dd = tmem + d + 16 * ks;
-          umma_f16_ts(dd, ahi, hi, id, ks > 0);
-          umma_f16_ts(dd, alo, hi, id, 1);
-          umma_f16_ts(dd, ahi, lo, id, 1);
-        }
-      };
-      for (int c = 0; c < nchunks; ++c) {
-        const int st = c % kStages;
-        const uint32_t ph = c & 1, sph = (c / kStages) & 1;
-        ChainStage& g = s.st[st];
-        if (!mbar_wait(&s.full[st], sph, status, kErrTimeoutMma, abort)) break;
-        if (!mbar_wait(&s.ready[st], sph, status, kErrTimeoutMma, abort)) break;
-        if (!mbar_wait(&s.s_ready, ph, status, kErrTimeoutMma, abort)) break;
-        tc_fence_after();
-        state_product(kColD1, g.k);
-        umma_commit(&s.d1_full);
-        if (c > 0 && !mbar_wait(&s.o_read, ph ^ 1, status, kErrTimeoutMma, abort)) break;
-        tc_fence_after();
-        state_product(kColD2, g.q);
-        umma_commit(&s.d2_full);
-        if (!mbar_wait(&s.r_ready, ph, status, kErrTimeoutMma, abort)) break;
-        tc_fence_after();
-        tri_product(kColD3, kColD1, g.item);
-        umma_commit(&s.d3_full);
-        if (!mbar_wait(&s.v_ready, ph, status, kErrTimeoutMma, abort)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const uint64_t db = sdesc_mn(smem_u32(g.k[0]) + ks * 2048, kC * 128);
-          const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
-          umma_f16_ts(tmem + kColDS, ahi, db, id128mn, ks > 0);
-          umma_f16_ts(tmem + kColDS, ahi + 16, db, id128mn, 1);
-        }
-        umma_commit(&s.ds_full);
-        if (!mbar_wait(&s.d2_read, ph, status, kErrTimeoutMma, abort)) break;
-        tc_fence_after();
-        tri_product(kColD2, kColD1, g.item + 2 * kTri);
-        umma_commit(&s.o_full);
-        umma_commit(&s.empty[st]);
+      for (int ks = 0; ks < 4; ++ks) {
+        const uint64_t db = sdesc_sw128(smem_u32(b)) + 2 * ks;
+        const uint32_t hi = tmem + kColS + g * 32 + ks * 8;
+        if (elect_one()) umma_f16_ts(tmem + d, hi, db, id64, g > 0 || ks > 0);
+        if (elect_one()) umma_f16_ts(tmem + d, hi + 64, db, id64, 1);
       }
-      umma_commit(&s.mma_done);
-      volatile int never = 0;
-      mbar_wait(&s.mma_done, 0, nullptr, 0, &never);
+    };
+    // D[128 x 64] = A B^T, B lower triangular in two pieces; A in two pieces of 16 columns per 32 tokens
+    auto tri_product = [&](uint32_t d, uint32_t acol, const uint8_t* b) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const int rows = kC - 16 * ks;
+        const uint32_t id = idesc_make(128, rows, 1), base = smem_u32(b) + tri_start(ks);
+        const uint64_t hi = sdesc_core(base, rows * 16), lo = sdesc_core(base + kTri, rows * 16);
+        const uint32_t ahi = tmem + acol + (ks >> 1) * 32 + (ks & 1) * 8, alo = ahi + 16, dd = tmem + d + 16 * ks;
+        if (elect_one()) umma_f16_ts(dd, ahi, hi, id, ks > 0);
+        if (elect_one()) umma_f16_ts(dd, alo, hi, id, 1);
+        if (elect_one()) umma_f16_ts(dd, ahi, lo, id, 1);
+      }
+    };
+    for (int c = 0; c < nchunks; ++c) {
+      const int st = c % kStages;
+      const uint32_t ph = c & 1, sph = (c / kStages) & 1;
+      ChainStage& g = s.st[st];
+      if (!wait(&s.full[st], sph) || !wait(&s.ready[st], sph)) break;
+      if (!wait(&s.s_ready[0], ph)) break;
+      state_product(kColD1, g.k[0], 0);
+      if (!wait(&s.s_ready[1], ph)) break;
+      state_product(kColD1, g.k[1], 1);
+      commit(&s.d1_full);
+      if (c > 0 && !wait(&s.o_read, ph ^ 1)) break;
+      state_product(kColD2, g.q[0], 0);
+      if (!wait(&s.r_ready, ph)) break;
+      tri_product(kColD3, kColD1, g.item);
+      commit(&s.d3_full);
+      state_product(kColD2, g.q[1], 1);
+      commit(&s.d2_full);
+      if (!wait(&s.v_ready, ph)) break;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const uint64_t db = sdesc_mn(smem_u32(g.k[b]) + ks * 2048, kC * 128);
+          const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
+          if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi, db, id64mn, ks > 0);
+          if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi + 16, db, id64mn, 1);
+        }
+        commit(&s.ds_full[b]);
+      }
+      if (!wait(&s.p_ready, ph) || !wait(&s.d2_read, ph)) break;
+      tri_product(kColD2, kColD1, g.item + 2 * kTri);
+      commit(&s.o_full);
+      commit(&s.empty[st]);
     }
+    commit(&s.mma_done);
+    volatile int never = 0;
+    mbar_wait(&s.mma_done, 0, nullptr, 0, &never);
   } else if (warp < 10) {
     // ---------------- state warps ----------------
     const int half = (warp - 2) >> 2, quad = warp & 3, v = quad * 32 + lane;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    float* gS = a.state + (((int64_t)slot * a.HV + h) * kDim + half * 64) * kDim + v;
+    float* gS = a.state + (((int64_t)slot * a.HV + h) * kDim + half * 32) * kDim + v;
     float S[64];
 #pragma unroll
-    for (int j = 0; j < 64; ++j) S[j] = gS[j * kDim];
+    for (int j = 0; j < 64; ++j) S[j] = gS[((j >> 5) * 64 + (j & 31)) * kDim];
     // 16 floats -> two bf16 pieces of 8 TMEM columns each
     auto store_pieces = [&](uint32_t hi_col, uint32_t lo_col, const float* x) {
       uint32_t hi[8], lo[8];
@@ -538,6 +689,13 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       for (int e = 0; e < 8; ++e) split2(x[2 * e], x[2 * e + 1], hi[e], lo[e]);
       tmem_st8(tl + hi_col, hi);
       tmem_st8(tl + lo_col, lo);
+    };
+    auto store_state = [&](int g) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t col = kColS + g * 32 + half * 16 + u * 8;
+        store_pieces(col, col + 64, S + 32 * g + 16 * u);
+      }
     };
     auto hand_over = [&](uint64_t* bar) {
       tmem_wait_st();
@@ -551,71 +709,97 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       tc_fence_after();
       return true;
     };
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      store_state(g);
+      hand_over(&s.s_ready[g]);
+    }
     bool ok = true;
     for (int c = 0; c < nchunks; ++c) {
       const int st = c % kStages, n = c == nchunks - 1 ? tail : kC;
       const uint32_t ph = c & 1;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) store_pieces(kColS + half * 32 + g * 8, kColS + 64 + half * 32 + g * 8, S + 16 * g);
-      hand_over(&s.s_ready);
-
+      float R[32];
       if (!(ok = wait(&s.full[st], (c / kStages) & 1))) break;
       const float* vec = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + half * 32;
-      const float decay = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri)[4 * kC];
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(vec + i);
+        const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) R[i + e] = __bfloat162float(s.st[st].v[half * 32 + i + e][v]) * bb[e];
+      }
       if (!(ok = wait(&s.d1_full, ph))) break;
-      float R[32];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         uint32_t d[16];
         tmem_ld16(tl + kColD1 + half * 32 + g * 16, d);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) R[16 * g + e] = __bfloat162float(s.st[st].v[half * 32 + 16 * g + e][v]) * vec[16 * g + e];
         tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = 16 * g + e;
-          R[i] = fmaf(-vec[kC + i], __uint_as_float(d[e]), R[i]);
-          if (half * 32 + i >= n) R[i] = 0.f;      // tokens past the request's end
+        for (int i = 0; i < 16; i += 4) {
+          const float4 c1 = *reinterpret_cast<const float4*>(vec + kC + 16 * g + i);
+          R[16 * g + i] = fmaf(-c1.x, __uint_as_float(d[i]), R[16 * g + i]);
+          R[16 * g + i + 1] = fmaf(-c1.y, __uint_as_float(d[i + 1]), R[16 * g + i + 1]);
+          R[16 * g + i + 2] = fmaf(-c1.z, __uint_as_float(d[i + 2]), R[16 * g + i + 2]);
+          R[16 * g + i + 3] = fmaf(-c1.w, __uint_as_float(d[i + 3]), R[16 * g + i + 3]);
         }
       }
-      // every column of this half is read before its pieces overwrite it
+      if (n < kC) {                                // tokens past the request's end
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (half * 32 + i >= n) R[i] = 0.f;
+      }
+      // every column of this half has been read before its pieces overwrite it
 #pragma unroll
       for (int g = 0; g < 2; ++g) store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
       hand_over(&s.r_ready);
 
       if (!(ok = wait(&s.d3_full, ph))) break;
-      {
-        uint32_t d[32];
-        tmem_ld32(tl + kColD3 + half * 32, d);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t d[16];
+        tmem_ld16(tl + kColD3 + half * 32 + g * 16, d);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) R[i] += __uint_as_float(d[i]);
+        for (int i = 0; i < 16; ++i) R[16 * g + i] += __uint_as_float(d[i]);
       }
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = R[16 * g + e] * vec[2 * kC + 16 * g + e];
+        for (int i = 0; i < 16; i += 4) {
+          const float4 c2 = *reinterpret_cast<const float4*>(vec + 2 * kC + 16 * g + i);
+          x[i] = R[16 * g + i] * c2.x, x[i + 1] = R[16 * g + i + 1] * c2.y;
+          x[i + 2] = R[16 * g + i + 2] * c2.z, x[i + 3] = R[16 * g + i + 3] * c2.w;
+        }
         store_pieces(kColD3 + half * 32 + g * 8, kColD3 + half * 32 + 16 + g * 8, x);
-        store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
       }
       hand_over(&s.v_ready);
+      const float decay = vec[4 * kC - half * 32];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
+      hand_over(&s.p_ready);
 
 #pragma unroll
-      for (int j = 0; j < 64; ++j) S[j] *= decay;
-      if (!(ok = wait(&s.ds_full, ph))) break;
-#pragma unroll
       for (int g = 0; g < 2; ++g) {
-        uint32_t d[32];
-        tmem_ld32(tl + kColDS + half * 64 + g * 32, d);
-        tmem_wait_ld();
+        if (!(ok = wait(&s.ds_full[g], ph))) break;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) S[32 * g + j] += __uint_as_float(d[j]);
+        for (int u = 0; u < 2; ++u) {
+          uint32_t d[16];
+          tmem_ld16(tl + kColDS + g * 64 + half * 32 + u * 16, d);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) S[32 * g + 16 * u + j] = fmaf(S[32 * g + 16 * u + j], decay, __uint_as_float(d[j]));
+        }
+        if (c + 1 < nchunks) {
+          store_state(g);
+          hand_over(&s.s_ready[g]);
+        }
       }
+      if (!ok) break;
     }
     if (ok) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j) gS[j * kDim] = S[j];
+      for (int j = 0; j < 64; ++j) gS[((j >> 5) * 64 + (j & 31)) * kDim] = S[j];
     }
   } else {
     // ---------------- output warps ----------------
@@ -635,32 +819,47 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     for (int c = 0; c < nchunks; ++c) {
       const int st = c % kStages, n = c == nchunks - 1 ? tail : kC;
       const uint32_t ph = c & 1;
-      float o[kC];
-      uint32_t d[32];
+      uint32_t o[kC];
       if (!wait(&s.full[st], (c / kStages) & 1)) break;
       if (!wait(&s.d2_full, ph)) break;
-      const float* c3 = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + 3 * kC;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        tmem_ld32(tl + kColD2 + g * 32, d);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[32 * g + i] = __uint_as_float(d[i]) * c3[32 * g + i];
-      }
+      tmem_ld32(tl + kColD2, *reinterpret_cast<uint32_t(*)[32]>(o));
+      tmem_ld32(tl + kColD2 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+      tmem_wait_ld();
       arrive(&s.d2_read);
       if (!wait(&s.o_full, ph)) break;
-      __nv_bfloat16* out = a.out + ((int64_t)(t0 + c * kC) * a.HV + h) * kDim + v;
+      const float* c3 = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + 3 * kC;
+      __nv_bfloat16 (*stage)[kDim] = s.st[st].v;      // v has been read: its place takes the chunk's output
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        tmem_ld32(tl + kColD2 + g * 32, d);
+      for (int g = 0; g < 4; ++g) {
+        uint32_t d[16];
+        tmem_ld16(tl + kColD2 + g * 16, d);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (32 * g + i < n) out[(int64_t)(32 * g + i) * a.HV * kDim] = __float2bfloat16(o[32 * g + i] + __uint_as_float(d[i]));
+        for (int i = 0; i < 16; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(c3 + 16 * g + i);
+          const float x0 = fmaf(f.x, __uint_as_float(o[16 * g + i]), __uint_as_float(d[i]));
+          const float x1 = fmaf(f.y, __uint_as_float(o[16 * g + i + 1]), __uint_as_float(d[i + 1]));
+          const float x2 = fmaf(f.z, __uint_as_float(o[16 * g + i + 2]), __uint_as_float(d[i + 2]));
+          const float x3 = fmaf(f.w, __uint_as_float(o[16 * g + i + 3]), __uint_as_float(d[i + 3]));
+          const __nv_bfloat162 a01 = __floats2bfloat162_rn(x0, x1), a23 = __floats2bfloat162_rn(x2, x3);
+          stage[16 * g + i][v] = a01.x, stage[16 * g + i + 1][v] = a01.y;
+          stage[16 * g + i + 2][v] = a23.x, stage[16 * g + i + 3][v] = a23.y;
+        }
       }
       arrive(&s.o_read);
+      fence_proxy_async_smem();
+      arrive(&s.o_staged);
+      if (!wait(&s.o_staged, ph)) break;
+      const int row = quad * 16 + lane;               // one token's 256 bytes per lane
+      if (lane < 16 && row < n) {
+        bulk_store(a.out + ((int64_t)(t0 + c * kC + row) * a.HV + h) * kDim, stage[row], kDim * 2);
+        bulk_commit();
+        bulk_wait_read0();
+      }
+      __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[st]);
     }
+    bulk_wait0();
   }
   tc_fence_before();
   __syncthreads();
@@ -702,7 +901,7 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
     return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
            t.stride(0) > 0 && t.stride(1) > 0;
   };
-  if (T <= kStepMean * R || !rows16(q) || !rows16(k) || !rows16(v)) {
+  if (T <= kStepMean * R || !rows16(q) || !rows16(k) || !rows16(v) || !rows16(out)) {
     gdn_step_kernel<<<dim3((unsigned)R, (unsigned)HV), 256, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     return;
@@ -720,14 +919,15 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   cudaGetDevice(&dev);
   static bool opted[64] = {};   // the opt-in belongs to each device's context
   TORCH_CHECK(dev < 64, "device index out of range");
-  constexpr int chain_smem = sizeof(ChainSmem) + 1024, prep_smem = sizeof(PrepSmem);
+  constexpr int chain_smem = sizeof(ChainSmem) + 1024;
   if (!opted[dev]) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(gdn_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, chain_smem));
-    C10_CUDA_CHECK(cudaFuncSetAttribute(gdn_prep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, prep_smem));
     opted[dev] = true;
   }
   uint8_t* it = items.data_ptr<uint8_t>();
-  gdn_prep_kernel<<<dim3((unsigned)n_items, (unsigned)HV), 128, prep_smem, stream>>>(a, it);
+  // value heads of one key head in turn share its loads and Gram matrices, where that leaves CTAs enough for the machine
+  const int rep = (int)(HV / HK), heads = n_items * HK >= 4 * 148 ? rep : 1;
+  gdn_prep_kernel<<<dim3((unsigned)n_items, (unsigned)(HV / heads)), 128, 0, stream>>>(a, it, heads);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   gdn_chain_kernel<<<dim3((unsigned)HV, (unsigned)R), kChainThreads, chain_smem, stream>>>(tk, tq, tv, a, it);
   C10_CUDA_KERNEL_LAUNCH_CHECK();

@@ -38,6 +38,8 @@ def _gdn_inputs(lens, hk, hv, seed=0, extra=0, kind="usual"):
         a["beta"].fill_(1.0)
     elif kind == "hard decay":          # single tokens that forget nearly everything, between ones that keep it
         a["g"] = torch.where(torch.rand(t, hv, generator=gen, device=DEV) < 0.1, -3000.0, a["g"] * 0.1)
+    elif kind == "resets":              # gates that close: the state starts anew there
+        a["g"][::7] = float("-inf")
     elif kind == "one key":             # every token writes to the same key: the chunk's system is as dense as it gets
         a["k"].copy_(a["k"][:1].clone().expand_as(a["k"]))
         a["beta"].fill_(1.0)
@@ -99,7 +101,7 @@ def test_gdn_chunked(lens, hk, hv):
     _gdn_check(_gdn_inputs(lens, hk, hv, seed=sum(lens) + hv))
 
 
-@pytest.mark.parametrize("kind", ["no decay", "hard decay", "one key", "zeros", "large"])
+@pytest.mark.parametrize("kind", ["no decay", "hard decay", "resets", "one key", "zeros", "large"])
 @pytest.mark.parametrize("lens", [[200, 70], [5, 1, 9]])
 def test_gdn_chunked_values(kind, lens):
     _gdn_check(_gdn_inputs(lens, 2, 4, seed=len(lens), kind=kind))
