@@ -476,9 +476,13 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 // The chain: one CTA per (request, value head). Everything is transposed, so that TMEM lanes are the 128 value columns
 // and the state never leaves the registers of the warps that own those lanes:
 //   warp 0       loader: k, q (128-byte swizzle), v tiles and the chunk's item, kStages ahead
-//   warp 1       TMEM owner; issues the products
-//   warps 2-9    state warps: a thread has lane v and the key columns g * 64 + half * 32 + 0..31, g = 0, 1, of S
-//   warps 10-13  output warps: a thread has lane v and the chunk's 64 tokens
+//   warp 1       TMEM owner; issues the products (warps 2 and 3 only fill the warpgroup)
+//   warps 4-11   state warps: a thread has lane v and the key columns g * 64 + half * 32 + 0..31, g = 0, 1, of S
+//   warps 12-15  output warps: 32 value columns and the chunk's 64 tokens each
+// Token columns of TMEM (D1 to D4) are read in 16 x 256-bit fragments: a thread has 8 pairs of neighbouring tokens instead
+// of 32, so its factors are a few 8-byte loads, v comes by transposing ldmatrix and the output leaves by stmatrix. (One
+// lane per value column, every token: 1500 shared-memory wavefronts a chunk, which were the chain's bound.)
+// Registers move from the first warpgroup to the state warps: 56 + 2 x 168 + 112 = 504 of the launch's 4 x 128.
 // Per chunk (A operands in TMEM, B operands in shared memory, fp32 accumulators in TMEM):
 //   D1 = S^T k^T                          S pieces written by the state warps
 //   D2 = S^T q^T
@@ -488,18 +492,18 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 //   D4 = V'^T P^T, o = c3 D2 + D4         c3 = e^b scale / |q|
 // The chain's latency bounds it: S -> D1 -> R -> D3 -> V' -> DS -> S. S goes through in two halves of 64 key columns, so
 // that converting one overlaps the products of the other; D2 and D4 fill the tensor core's gaps.
-// TMEM columns: S pieces 128 | D1, then R, then V' pieces 64 | D2, then D4 64 | D3, then V' c2 pieces 64 | DS 128.
+// TMEM columns: S pieces 128 | D1, then R, then V' pieces 64 | D2 64 | D3, then V' c2 pieces 64 | DS 128 | D4 64.
 // A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
 // ------------------------------------------------------------------------------------------------
 constexpr int kStages = 3;
-constexpr int kChainThreads = 14 * 32;
-constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColDS = 320, kTmemCols = 512;
+constexpr int kChainThreads = 16 * 32;
+constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColDS = 320, kColD4 = 448, kTmemCols = 512;
 constexpr int kStageTx = 3 * kC * kDim * 2 + kItemBytes;
 
 struct ChainStage {
   uint8_t k[2][kC * 128];       // key dimensions 0-63 and 64-127, 128 bytes per token
   uint8_t q[2][kC * 128];
-  __nv_bfloat16 v[kC][kDim];
+  uint8_t v[2][kC * 128];       // value columns 0-63 and 64-127; later the chunk's output
   uint8_t item[(kItemBytes + 1023) / 1024 * 1024];
 };
 struct ChainSmem {
@@ -523,6 +527,47 @@ __device__ __forceinline__ uint64_t sdesc_core(uint32_t saddr, uint32_t lbo) {
          static_cast<uint64_t>(128 >> 4) << 32 | static_cast<uint64_t>(1) << 46;
 }
 
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ float2 lds2(uint32_t addr) {
+  float2 f;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(addr));
+  return f;
+}
+// 8 x 8 tiles of 16-bit elements, transposed on the way: of tile j (register j) lane l has row l / 4, columns 2 (l % 4)
+// and 2 (l % 4) + 1, where the tile's columns are the eight rows in memory that lanes 8 j .. 8 j + 7 point at
+__device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void stmatrix_x4_t(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// 16 TMEM lanes x 32 columns: for m = 0..3 lane l gets columns 8 m + 2 (l % 4), + 1 of TMEM lanes l / 4 and l / 4 + 8
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// 16 TMEM lanes x 16 columns: for m = 0..3 lane l has column 4 m + l % 4 of TMEM lanes l / 4 and l / 4 + 8
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 // 1-D bulk copy of global memory into this CTA's shared memory, counted on `bar`
 __device__ __forceinline__ void bulk_load(uint64_t* bar, void* dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
@@ -530,9 +575,43 @@ __device__ __forceinline__ void bulk_load(uint64_t* bar, void* dst, const void* 
                : "memory");
 }
 
+// Bounded wait, kept to a few instructions: the chain's loops have to stay in the instruction cache (with a timer and a
+// status write at each of its 20 waits the kernel was 115 KB of code and 1.5 times as slow). False: the bound was
+// reached or another warp gave up; give_up() then reports it once.
+__device__ __forceinline__ bool mbar_wait_n(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < (1 << 20); ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+  }
+  return false;
+}
+// The same without going to sleep between tries, for the one warp whose every wait is on the chain.
+__device__ __forceinline__ bool mbar_spin_n(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+  for (int i = 0; i < (1 << 26); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((i & 255) == 255 && *abort) return false;
+  }
+  return false;
+}
+__device__ __noinline__ void give_up(int* status, int code, volatile int* abort) {
+  if (!*abort) atomicCAS(status, 0, code);
+  *abort = 1;
+}
+
 __global__ void __launch_bounds__(kChainThreads, 1)
     gdn_chain_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ,
-                     const __grid_constant__ CUtensorMap tmV, const GdnArgs a, const uint8_t* __restrict__ items) {
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const GdnArgs a,
+                     const uint8_t* __restrict__ items) {
   extern __shared__ uint8_t smem_raw[];
   ChainSmem& s = *reinterpret_cast<ChainSmem*>(smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023));
   const int warp = warp_id(), lane = lane_id();
@@ -546,7 +625,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.ready[i], 1);
-      mbar_init(&s.empty[i], 5);       // the tensor core and the four output warps
+      mbar_init(&s.empty[i], 2);       // the tensor core, and the output's way out
     }
     for (uint64_t* b : {&s.s_ready[0], &s.s_ready[1], &s.r_ready, &s.v_ready, &s.p_ready}) mbar_init(b, 8);
     for (uint64_t* b : {&s.d2_read, &s.o_read, &s.o_staged}) mbar_init(b, 4);
@@ -565,16 +644,17 @@ __global__ void __launch_bounds__(kChainThreads, 1)
   volatile int* abort = &s.abort;
   int* status = a.status;
 
+  if (warp < 4) regs_down<56>();
   if (warp == 0) {
     // ---------------- loader ----------------
     const int item0 = first_item(a, r);
     int issued = 0;
+    bool ok = true;
     for (int c = 0; c < nchunks; ++c) {
       const int st = c % kStages;
       const uint32_t ph = (c / kStages) & 1;
       ChainStage& g = s.st[st];
-      const bool ok = mbar_wait(&s.empty[st], ph ^ 1, status, kErrTimeoutProducer, abort);
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait_n(&s.empty[st], ph ^ 1, abort)))) break;
       if (lane == 0) {
         const int t = t0 + c * kC;
         mbar_arrive_expect_tx(&s.full[st], kStageTx);
@@ -583,14 +663,14 @@ __global__ void __launch_bounds__(kChainThreads, 1)
         bulk_load(&s.full[st], g.item, items + ((int64_t)(item0 + c) * a.HV + h) * kItemBytes, kItemBytes);
         tma_load_3d(&tmQ, &s.full[st], g.q[0], 0, hk, t);
         tma_load_3d(&tmQ, &s.full[st], g.q[1], 64, hk, t);
-        tma_load_3d(&tmV, &s.full[st], g.v, 0, h, t);
+        tma_load_3d(&tmV, &s.full[st], g.v[0], 0, h, t);
+        tma_load_3d(&tmV, &s.full[st], g.v[1], 64, h, t);
       }
       ++issued;
       if (c == nchunks - 1 && tail < kC) {
         // k rows past the request's end belong to another request: the update multiplies them by 0, so they have to
         // be finite
-        const bool in = mbar_wait(&s.full[st], ph, status, kErrTimeoutProducer, abort);
-        if (!__all_sync(0xffffffffu, in)) break;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait_n(&s.full[st], ph, abort)))) break;
         for (int x = lane; x < (kC - tail) * 16; x += 32)
           *reinterpret_cast<uint4*>(&g.k[x & 1][(tail + (x >> 4)) * 128 + (x >> 1 & 7) * 16]) = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
@@ -598,16 +678,16 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       }
       if (lane == 0) mbar_arrive(&s.ready[st]);
     }
+    if (!ok) give_up(status, kErrTimeoutProducer, abort);
     // the copies in flight land before the CTA may exit (bounded)
     volatile int never = 0;
-    for (int c = max(0, issued - kStages); c < issued; ++c) mbar_wait(&s.full[c % kStages], (c / kStages) & 1, nullptr, 0, &never);
+    for (int c = max(0, issued - kStages); c < issued; ++c) mbar_wait_n(&s.full[c % kStages], (c / kStages) & 1, &never);
   } else if (warp == 1) {
     // ---------------- product issuer: the whole warp walks the loop, one elected lane issues. (A branch for one lane
     // around the loop keeps descriptors out of the uniform registers: 78 instead of 32 cycles a 64-column product.)
     constexpr uint32_t id64 = idesc_make(128, 64, 1), id64mn = id64 | (1u << 16);
     auto wait = [&](uint64_t* bar, uint32_t ph) {
-      const bool ok = mbar_wait(bar, ph, status, kErrTimeoutMma, abort);
-      if (!__all_sync(0xffffffffu, ok)) return false;
+      if (!__all_sync(0xffffffffu, mbar_spin_n(bar, ph, abort))) return false;
       tc_fence_after();
       return true;
     };
@@ -637,46 +717,57 @@ __global__ void __launch_bounds__(kChainThreads, 1)
         if (elect_one()) umma_f16_ts(dd, ahi, lo, id, 1);
       }
     };
-    for (int c = 0; c < nchunks; ++c) {
+    // D[128 x 64] = (V' c2)^T k over the chunk's tokens, key dimensions 64 b .. 64 b + 63 (k MN-major)
+    auto state_update = [&](ChainStage& g, int b) {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const uint64_t db = sdesc_mn(smem_u32(g.k[b]) + ks * 2048, kC * 128);
+        const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
+        if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi, db, id64mn, ks > 0);
+        if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi + 16, db, id64mn, 1);
+      }
+      commit(&s.ds_full[b]);
+    };
+    int c = 0;
+    for (; c < nchunks; ++c) {
       const int st = c % kStages;
-      const uint32_t ph = c & 1, sph = (c / kStages) & 1;
+      const uint32_t ph = c & 1;
       ChainStage& g = s.st[st];
-      if (!wait(&s.full[st], sph) || !wait(&s.ready[st], sph)) break;
+      if (c == 0 && (!wait(&s.full[0], 0) || !wait(&s.ready[0], 0))) break;
       if (!wait(&s.s_ready[0], ph)) break;
       state_product(kColD1, g.k[0], 0);
       if (!wait(&s.s_ready[1], ph)) break;
       state_product(kColD1, g.k[1], 1);
       commit(&s.d1_full);
-      if (c > 0 && !wait(&s.o_read, ph ^ 1)) break;
+      if (c > 0 && !wait(&s.d2_read, ph ^ 1)) break;
       state_product(kColD2, g.q[0], 0);
       if (!wait(&s.r_ready, ph)) break;
       tri_product(kColD3, kColD1, g.item);
       commit(&s.d3_full);
       state_product(kColD2, g.q[1], 1);
       commit(&s.d2_full);
-      if (!wait(&s.v_ready, ph)) break;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const uint64_t db = sdesc_mn(smem_u32(g.k[b]) + ks * 2048, kC * 128);
-          const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
-          if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi, db, id64mn, ks > 0);
-          if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi + 16, db, id64mn, 1);
-        }
-        commit(&s.ds_full[b]);
+      if (c + 1 < nchunks) {                             // the next chunk's tiles, while there is time
+        const int nst = (c + 1) % kStages;
+        const uint32_t nph = ((c + 1) / kStages) & 1;
+        if (!wait(&s.full[nst], nph) || !wait(&s.ready[nst], nph)) break;
       }
-      if (!wait(&s.p_ready, ph) || !wait(&s.d2_read, ph)) break;
-      tri_product(kColD2, kColD1, g.item + 2 * kTri);
+      if (!wait(&s.v_ready, ph)) break;
+      state_update(g, 0);
+      state_update(g, 1);
+      if (!wait(&s.p_ready, ph)) break;
+      if (c > 0 && !wait(&s.o_read, ph ^ 1)) break;
+      tri_product(kColD4, kColD1, g.item + 2 * kTri);
       commit(&s.o_full);
       commit(&s.empty[st]);
     }
+    if (c < nchunks) give_up(status, kErrTimeoutMma, abort);
     commit(&s.mma_done);
     volatile int never = 0;
-    mbar_wait(&s.mma_done, 0, nullptr, 0, &never);
-  } else if (warp < 10) {
+    mbar_wait_n(&s.mma_done, 0, &never);
+  } else if (warp >= 4 && warp < 12) {
     // ---------------- state warps ----------------
-    const int half = (warp - 2) >> 2, quad = warp & 3, v = quad * 32 + lane;
+    regs_up<168>();
+    const int half = (warp - 4) >> 2, quad = warp & 3, v = quad * 32 + lane;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     float* gS = a.state + (((int64_t)slot * a.HV + h) * kDim + half * 32) * kDim + v;
     float S[64];
@@ -690,6 +781,21 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       tmem_st8(tl + hi_col, hi);
       tmem_st8(tl + lo_col, lo);
     };
+    // 16 value columns x this half's 32 tokens -> two bf16 pieces of 16 TMEM columns each
+    auto store_tokens = [&](int u, uint32_t col, const float (&x)[4][4]) {
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        split2(x[m][0], x[m][1], hi[2 * m], lo[2 * m]);
+        split2(x[m][2], x[m][3], hi[2 * m + 1], lo[2 * m + 1]);
+      }
+      tmem_st_frag(tl + (u << 20) + col + half * 32, hi);
+      tmem_st_frag(tl + (u << 20) + col + half * 32 + 16, lo);
+    };
+    const int t = lane & 3;
+    // v tile (token row % 8 = lane % 8, value columns quad * 32 + 8 (lane / 8) ..) of a group of eight tokens
+    const int vc = quad * 4 + (lane >> 3);
+    const uint32_t vtile = (vc >> 3) * kC * 128 + (lane & 7) * 128 + (((vc & 7) ^ (lane & 7)) << 4);
     auto store_state = [&](int g) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -704,8 +810,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       if (lane == 0) mbar_arrive(bar);
     };
     auto wait = [&](uint64_t* bar, uint32_t ph) {
-      const bool ok = mbar_wait(bar, ph, status, kErrTimeoutEpilogue, abort);
-      if (!__all_sync(0xffffffffu, ok)) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait_n(bar, ph, abort))) return false;
       tc_fence_after();
       return true;
     };
@@ -714,82 +819,99 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       store_state(g);
       hand_over(&s.s_ready[g]);
     }
-    bool ok = true;
-    for (int c = 0; c < nchunks; ++c) {
-      const int st = c % kStages, n = c == nchunks - 1 ? tail : kC;
-      const uint32_t ph = c & 1;
-      float R[32];
-      if (!(ok = wait(&s.full[st], (c / kStages) & 1))) break;
-      const float* vec = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + half * 32;
+    // R[u][m]: tokens half * 32 + 8 m + 2 t, + 1 of value columns quad * 32 + 16 u + lane / 4 (first two) and + 8
+    float R[2][4][4], decay = 0.f;
+    float2 f[4];
+    uint32_t vec = 0;
+    auto load_v = [&](int c) {         // R = beta v, f = c1 of chunk c
+      const int st = c % kStages;
+      if (!wait(&s.full[st], (c / kStages) & 1)) return false;
+      vec = smem_u32(s.st[st].item) + 4 * kTri + (half * 32 + 2 * t) * 4;
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(vec + i);
-        const float bb[4] = {b.x, b.y, b.z, b.w};
+      for (int m = 0; m < 4; ++m) f[m] = lds2(vec + m * 32);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) R[i + e] = __bfloat162float(s.st[st].v[half * 32 + i + e][v]) * bb[e];
+      for (int m = 0; m < 4; ++m) {
+        uint32_t x[4];
+        ldmatrix_x4_t(x, smem_u32(s.st[st].v) + vtile + (half * 32 + 8 * m) * 128);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = unpack_bf16x2(x[e]);
+          R[e >> 1][m][(e & 1) * 2] = y.x * f[m].x;
+          R[e >> 1][m][(e & 1) * 2 + 1] = y.y * f[m].y;
+        }
       }
-      if (!(ok = wait(&s.d1_full, ph))) break;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t d[16];
-        tmem_ld16(tl + kColD1 + half * 32 + g * 16, d);
+      for (int m = 0; m < 4; ++m) f[m] = lds2(vec + kC * 4 + m * 32);
+      return true;
+    };
+    bool ok = load_v(0);
+    for (int c = 0; ok && c < nchunks; ++c) {
+      const int n = c == nchunks - 1 ? tail : kC;
+      const uint32_t ph = c & 1;
+      if (!(ok = wait(&s.d1_full, ph))) break;
+      {
+        uint32_t d[2][16];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) tmem_ld_frag(tl + (u << 20) + kColD1 + half * 32, d[u]);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 c1 = *reinterpret_cast<const float4*>(vec + kC + 16 * g + i);
-          R[16 * g + i] = fmaf(-c1.x, __uint_as_float(d[i]), R[16 * g + i]);
-          R[16 * g + i + 1] = fmaf(-c1.y, __uint_as_float(d[i + 1]), R[16 * g + i + 1]);
-          R[16 * g + i + 2] = fmaf(-c1.z, __uint_as_float(d[i + 2]), R[16 * g + i + 2]);
-          R[16 * g + i + 3] = fmaf(-c1.w, __uint_as_float(d[i + 3]), R[16 * g + i + 3]);
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              R[u][m][e] = fmaf(e & 1 ? -f[m].y : -f[m].x, __uint_as_float(d[u][4 * m + e]), R[u][m][e]);
       }
       if (n < kC) {                                // tokens past the request's end
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (half * 32 + i >= n) R[i] = 0.f;
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (half * 32 + 8 * m + 2 * t + (e & 1) >= n) R[u][m][e] = 0.f;
       }
       // every column of this half has been read before its pieces overwrite it
 #pragma unroll
-      for (int g = 0; g < 2; ++g) store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
+      for (int u = 0; u < 2; ++u) store_tokens(u, kColD1, R[u]);
       hand_over(&s.r_ready);
 
-      if (!(ok = wait(&s.d3_full, ph))) break;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t d[16];
-        tmem_ld16(tl + kColD3 + half * 32 + g * 16, d);
+      for (int m = 0; m < 4; ++m) f[m] = lds2(vec + 2 * kC * 4 + m * 32);
+      if (!(ok = wait(&s.d3_full, ph))) break;
+      {
+        uint32_t d[2][16];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) tmem_ld_frag(tl + (u << 20) + kColD3 + half * 32, d[u]);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) R[16 * g + i] += __uint_as_float(d[i]);
-      }
+        for (int u = 0; u < 2; ++u) {
+          float x[4][4];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        float x[16];
+          for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 c2 = *reinterpret_cast<const float4*>(vec + 2 * kC + 16 * g + i);
-          x[i] = R[16 * g + i] * c2.x, x[i + 1] = R[16 * g + i + 1] * c2.y;
-          x[i + 2] = R[16 * g + i + 2] * c2.z, x[i + 3] = R[16 * g + i + 3] * c2.w;
+            for (int e = 0; e < 4; ++e) {
+              R[u][m][e] += __uint_as_float(d[u][4 * m + e]);
+              x[m][e] = R[u][m][e] * (e & 1 ? f[m].y : f[m].x);
+            }
+          store_tokens(u, kColD3, x);
         }
-        store_pieces(kColD3 + half * 32 + g * 8, kColD3 + half * 32 + 16 + g * 8, x);
       }
       hand_over(&s.v_ready);
-      const float decay = vec[4 * kC - half * 32];
+      decay = lds2(vec + (4 * kC - half * 32 - 2 * t) * 4).x;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) store_pieces(kColD1 + half * 32 + g * 8, kColD1 + half * 32 + 16 + g * 8, R + 16 * g);
+      for (int u = 0; u < 2; ++u) store_tokens(u, kColD1, R[u]);
       hand_over(&s.p_ready);
+      if (c + 1 < nchunks && !(ok = load_v(c + 1))) break;
 
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         if (!(ok = wait(&s.ds_full[g], ph))) break;
+        uint32_t d[32];
+        tmem_ld32(tl + kColDS + g * 64 + half * 32, d);
+        tmem_wait_ld();
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t d[16];
-          tmem_ld16(tl + kColDS + g * 64 + half * 32 + u * 16, d);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) S[32 * g + 16 * u + j] = fmaf(S[32 * g + 16 * u + j], decay, __uint_as_float(d[j]));
-        }
+        for (int j = 0; j < 32; ++j) S[32 * g + j] = fmaf(S[32 * g + j], decay, __uint_as_float(d[j]));
         if (c + 1 < nchunks) {
           store_state(g);
           hand_over(&s.s_ready[g]);
@@ -797,17 +919,19 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       }
       if (!ok) break;
     }
-    if (ok) {
+    if (!ok) {
+      give_up(status, kErrTimeoutEpilogue, abort);
+    } else {
 #pragma unroll
       for (int j = 0; j < 64; ++j) gS[((j >> 5) * 64 + (j & 31)) * kDim] = S[j];
     }
-  } else {
+  } else if (warp >= 12) {
     // ---------------- output warps ----------------
-    const int quad = warp & 3, v = quad * 32 + lane;
+    regs_down<112>();
+    const int quad = warp & 3;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     auto wait = [&](uint64_t* bar, uint32_t ph) {
-      const bool ok = mbar_wait(bar, ph, status, kErrTimeoutEpilogue, abort);
-      if (!__all_sync(0xffffffffu, ok)) return false;
+      if (!__all_sync(0xffffffffu, mbar_wait_n(bar, ph, abort))) return false;
       tc_fence_after();
       return true;
     };
@@ -816,50 +940,73 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    for (int c = 0; c < nchunks; ++c) {
+    const int vc = quad * 4 + (lane >> 3), t = lane & 3;
+    const uint32_t vtile = (vc >> 3) * kC * 128 + (lane & 7) * 128 + (((vc & 7) ^ (lane & 7)) << 4);
+    int c = 0;
+    for (; c < nchunks; ++c) {
       const int st = c % kStages, n = c == nchunks - 1 ? tail : kC;
       const uint32_t ph = c & 1;
-      uint32_t o[kC];
+      uint32_t o[2][2][16];      // [32 tokens][16 value columns]
       if (!wait(&s.full[st], (c / kStages) & 1)) break;
       if (!wait(&s.d2_full, ph)) break;
-      tmem_ld32(tl + kColD2, *reinterpret_cast<uint32_t(*)[32]>(o));
-      tmem_ld32(tl + kColD2 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) tmem_ld_frag(tl + (u << 20) + kColD2 + g * 32, o[g][u]);
       tmem_wait_ld();
       arrive(&s.d2_read);
+      if (c > 0 && warp == 12) {                       // the last chunk's output has left shared memory
+        if (lane == 0) {
+          bulk_wait_read0();
+          mbar_arrive(&s.empty[(c - 1) % kStages]);
+        }
+        __syncwarp();
+      }
       if (!wait(&s.o_full, ph)) break;
-      const float* c3 = reinterpret_cast<const float*>(s.st[st].item + 4 * kTri) + 3 * kC;
-      __nv_bfloat16 (*stage)[kDim] = s.st[st].v;      // v has been read: its place takes the chunk's output
+      const uint32_t c3 = smem_u32(s.st[st].item) + 4 * kTri + (3 * kC + 2 * t) * 4;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t d[16];
-        tmem_ld16(tl + kColD2 + g * 16, d);
+      for (int g = 0; g < 2; ++g) {
+        uint32_t d[2][16];
+        float2 f[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) tmem_ld_frag(tl + (u << 20) + kColD4 + g * 32, d[u]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) f[m] = lds2(c3 + (32 * g + 8 * m) * 4);
         tmem_wait_ld();
+        if (g == 1) arrive(&s.o_read);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(c3 + 16 * g + i);
-          const float x0 = fmaf(f.x, __uint_as_float(o[16 * g + i]), __uint_as_float(d[i]));
-          const float x1 = fmaf(f.y, __uint_as_float(o[16 * g + i + 1]), __uint_as_float(d[i + 1]));
-          const float x2 = fmaf(f.z, __uint_as_float(o[16 * g + i + 2]), __uint_as_float(d[i + 2]));
-          const float x3 = fmaf(f.w, __uint_as_float(o[16 * g + i + 3]), __uint_as_float(d[i + 3]));
-          const __nv_bfloat162 a01 = __floats2bfloat162_rn(x0, x1), a23 = __floats2bfloat162_rn(x2, x3);
-          stage[16 * g + i][v] = a01.x, stage[16 * g + i + 1][v] = a01.y;
-          stage[16 * g + i + 2][v] = a23.x, stage[16 * g + i + 3][v] = a23.y;
+        for (int m = 0; m < 4; ++m) {
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int u = e >> 1, k = 4 * m + (e & 1) * 2;
+            x[e] = pack_bf16x2(fmaf(f[m].x, __uint_as_float(o[g][u][k]), __uint_as_float(d[u][k])),
+                               fmaf(f[m].y, __uint_as_float(o[g][u][k + 1]), __uint_as_float(d[u][k + 1])));
+          }
+          // v has been read: its place takes the output, in the same swizzled form
+          stmatrix_x4_t(smem_u32(s.st[st].v) + vtile + (32 * g + 8 * m) * 128, x);
         }
       }
-      arrive(&s.o_read);
       fence_proxy_async_smem();
       arrive(&s.o_staged);
       if (!wait(&s.o_staged, ph)) break;
-      const int row = quad * 16 + lane;               // one token's 256 bytes per lane
-      if (lane < 16 && row < n) {
-        bulk_store(a.out + ((int64_t)(t0 + c * kC + row) * a.HV + h) * kDim, stage[row], kDim * 2);
-        bulk_commit();
-        bulk_wait_read0();
+      const int tok = t0 + c * kC;
+      if (n == kC) {
+        if (warp == 12 && lane == 0) {
+          tma_store_3d(&tmO, s.st[st].v[0], 0, h, tok);
+          tma_store_3d(&tmO, s.st[st].v[1], 64, h, tok);
+          bulk_commit();
+        }
+      } else {                                         // the last rows are not this request's
+        for (int x = (warp - 12) * 32 + lane; x < n * 16; x += 128) {
+          const int row = x >> 4, cc = x & 15;
+          const uint4 val = *reinterpret_cast<const uint4*>(&s.st[st].v[cc >> 3][row * 128 + (((cc & 7) ^ (row & 7)) << 4)]);
+          *reinterpret_cast<uint4*>(a.out + ((int64_t)(tok + row) * a.HV + h) * kDim + cc * 8) = val;
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.empty[st]);
     }
-    bulk_wait0();
+    if (c < nchunks) give_up(status, kErrTimeoutEpilogue, abort);
+    if (warp == 12 && lane == 0) bulk_wait0();
   }
   tc_fence_before();
   __syncthreads();
@@ -909,12 +1056,11 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   TORCH_CHECK(R < 65536, "at most 65535 requests");
   const int64_t n_items = T / kC + R;
   torch::Tensor items = torch::empty({n_items * HV * kItemBytes}, q.options().dtype(at::kByte));
-  auto map = [&](const torch::Tensor& t, int64_t heads, uint32_t box, CUtensorMapSwizzle sw) {
-    return make_tmap_3d(t.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kDim, heads, T, t.stride(1) * 2, t.stride(0) * 2, box, 1,
-                        kC, sw);
+  auto map = [&](const torch::Tensor& t, int64_t heads) {
+    return make_tmap_3d(t.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kDim, heads, T, t.stride(1) * 2, t.stride(0) * 2, 64, 1, kC,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
   };
-  const CUtensorMap tk = map(k, HK, 64, CU_TENSOR_MAP_SWIZZLE_128B), tq = map(q, HK, 64, CU_TENSOR_MAP_SWIZZLE_128B),
-                    tv = map(v, HV, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+  const CUtensorMap tk = map(k, HK), tq = map(q, HK), tv = map(v, HV), to = map(out, HV);
   int dev = 0;
   cudaGetDevice(&dev);
   static bool opted[64] = {};   // the opt-in belongs to each device's context
@@ -929,7 +1075,7 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   const int rep = (int)(HV / HK), heads = n_items * HK >= 4 * 148 ? rep : 1;
   gdn_prep_kernel<<<dim3((unsigned)n_items, (unsigned)(HV / heads)), 128, 0, stream>>>(a, it, heads);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  gdn_chain_kernel<<<dim3((unsigned)HV, (unsigned)R), kChainThreads, chain_smem, stream>>>(tk, tq, tv, a, it);
+  gdn_chain_kernel<<<dim3((unsigned)HV, (unsigned)R), kChainThreads, chain_smem, stream>>>(tk, tq, tv, to, a, it);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
