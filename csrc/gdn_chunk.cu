@@ -41,7 +41,10 @@ __device__ __forceinline__ bool request(const GdnArgs& a, int r, int& t0, int& t
   return ok;
 }
 
-constexpr int kStepMean = 16;            // mean tokens per request up to which tokens are taken one by one
+// Mean tokens per request up to which tokens are taken one by one. Measured, us by steps / by chunks: 1 request x 8 heads,
+// 16 tokens 14.5 / 16.5, 24 tokens 20.6 / 16.5; 64 requests x 16 heads, 8 tokens 58 / 78, 12 tokens 86 / 76; 200 x 32,
+// 4 tokens 331 / 429, 12 tokens 612 / 438: a step costs each wave of CTAs 0.5 us, the chunk form each wave its set-up.
+constexpr int kStepMeanOneWave = 16, kStepMean = 8;
 constexpr int kStepTokens = 16;          // tokens whose q and k are normalised together
 constexpr int kHalf = kDim / 2;
 constexpr int kRowPad = kDim + 8;        // the second half starts 4 floats later: both halves' reads miss each other's banks
@@ -491,13 +494,13 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 //   DS = (V' c2)^T k, S = e^(b_C) S + DS  c2 = e^(b_C - b) / |k|
 //   D4 = V'^T P^T, o = c3 D2 + D4         c3 = e^b scale / |q|
 // The chain's latency bounds it: S -> D1 -> R -> D3 -> V' -> DS -> S. S goes through in two halves of 64 key columns, so
-// that converting one overlaps the products of the other; D2 and D4 fill the tensor core's gaps.
-// TMEM columns: S pieces 128 | D1, then R, then V' pieces 64 | D2 64 | D3, then V' c2 pieces 64 | DS 128 | D4 64.
+// that converting one overlaps the products of the other; D2 and the last chunk's D4 run while the state warps work.
+// TMEM columns: DS, then S pieces 128 | D1, then R 64 | D2 64 | D3, then V' c2 pieces 64 | V' pieces 64 | D4 64.
 // A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
 // ------------------------------------------------------------------------------------------------
 constexpr int kStages = 3;
 constexpr int kChainThreads = 16 * 32;
-constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColDS = 320, kColD4 = 448, kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColV = 320, kColD4 = 384, kTmemCols = 512;
 constexpr int kStageTx = 3 * kC * kDim * 2 + kItemBytes;
 
 struct ChainStage {
@@ -699,9 +702,9 @@ __global__ void __launch_bounds__(kChainThreads, 1)
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const uint64_t db = sdesc_sw128(smem_u32(b)) + 2 * ks;
-        const uint32_t hi = tmem + kColS + g * 32 + ks * 8;
+        const uint32_t hi = tmem + kColS + g * 64 + (ks >> 1) * 32 + (ks & 1) * 8;
         if (elect_one()) umma_f16_ts(tmem + d, hi, db, id64, g > 0 || ks > 0);
-        if (elect_one()) umma_f16_ts(tmem + d, hi + 64, db, id64, 1);
+        if (elect_one()) umma_f16_ts(tmem + d, hi + 16, db, id64, 1);
       }
     };
     // D[128 x 64] = A B^T, B lower triangular in two pieces; A in two pieces of 16 columns per 32 tokens
@@ -723,10 +726,17 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       for (int ks = 0; ks < 4; ++ks) {
         const uint64_t db = sdesc_mn(smem_u32(g.k[b]) + ks * 2048, kC * 128);
         const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
-        if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi, db, id64mn, ks > 0);
-        if (elect_one()) umma_f16_ts(tmem + kColDS + 64 * b, ahi + 16, db, id64mn, 1);
+        if (elect_one()) umma_f16_ts(tmem + kColS + 64 * b, ahi, db, id64mn, ks > 0);
+        if (elect_one()) umma_f16_ts(tmem + kColS + 64 * b, ahi + 16, db, id64mn, 1);
       }
       commit(&s.ds_full[b]);
+    };
+    auto output_product = [&](int c) {               // D4 of chunk c, the last use of its tiles
+      if (!wait(&s.p_ready, c & 1) || (c > 0 && !wait(&s.o_read, (c & 1) ^ 1))) return false;
+      tri_product(kColD4, kColV, s.st[c % kStages].item + 2 * kTri);
+      commit(&s.o_full);
+      commit(&s.empty[c % kStages]);
+      return true;
     };
     int c = 0;
     for (; c < nchunks; ++c) {
@@ -739,7 +749,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       if (!wait(&s.s_ready[1], ph)) break;
       state_product(kColD1, g.k[1], 1);
       commit(&s.d1_full);
-      if (c > 0 && !wait(&s.d2_read, ph ^ 1)) break;
+      if (c > 0 && (!output_product(c - 1) || !wait(&s.d2_read, ph ^ 1))) break;
       state_product(kColD2, g.q[0], 0);
       if (!wait(&s.r_ready, ph)) break;
       tri_product(kColD3, kColD1, g.item);
@@ -754,12 +764,8 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       if (!wait(&s.v_ready, ph)) break;
       state_update(g, 0);
       state_update(g, 1);
-      if (!wait(&s.p_ready, ph)) break;
-      if (c > 0 && !wait(&s.o_read, ph ^ 1)) break;
-      tri_product(kColD4, kColD1, g.item + 2 * kTri);
-      commit(&s.o_full);
-      commit(&s.empty[st]);
     }
+    if (c == nchunks && !output_product(nchunks - 1)) --c;
     if (c < nchunks) give_up(status, kErrTimeoutMma, abort);
     commit(&s.mma_done);
     volatile int never = 0;
@@ -799,8 +805,8 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     auto store_state = [&](int g) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t col = kColS + g * 32 + half * 16 + u * 8;
-        store_pieces(col, col + 64, S + 32 * g + 16 * u);
+        const uint32_t col = kColS + g * 64 + half * 32 + u * 8;     // where this thread's part of DS was
+        store_pieces(col, col + 16, S + 32 * g + 16 * u);
       }
     };
     auto hand_over = [&](uint64_t* bar) {
@@ -823,31 +829,34 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     float R[2][4][4], decay = 0.f;
     float2 f[4];
     uint32_t vec = 0;
-    auto load_v = [&](int c) {         // R = beta v, f = c1 of chunk c
+    uint32_t raw[4][4];                // v of the next chunk as it is in memory
+    auto load_v = [&](int c) {
       const int st = c % kStages;
-      if (!wait(&s.full[st], (c / kStages) & 1)) return false;
-      vec = smem_u32(s.st[st].item) + 4 * kTri + (half * 32 + 2 * t) * 4;
+      if (!__all_sync(0xffffffffu, mbar_wait_n(&s.full[st], (c / kStages) & 1, abort))) return false;
+#pragma unroll
+      for (int m = 0; m < 4; ++m) ldmatrix_x4_t(raw[m], smem_u32(s.st[st].v) + vtile + (half * 32 + 8 * m) * 128);
+      return true;
+    };
+    auto start_chunk = [&](int c) {    // R = beta v, f = c1
+      vec = smem_u32(s.st[c % kStages].item) + 4 * kTri + (half * 32 + 2 * t) * 4;
 #pragma unroll
       for (int m = 0; m < 4; ++m) f[m] = lds2(vec + m * 32);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        uint32_t x[4];
-        ldmatrix_x4_t(x, smem_u32(s.st[st].v) + vtile + (half * 32 + 8 * m) * 128);
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 y = unpack_bf16x2(x[e]);
+          const float2 y = unpack_bf16x2(raw[m][e]);
           R[e >> 1][m][(e & 1) * 2] = y.x * f[m].x;
           R[e >> 1][m][(e & 1) * 2 + 1] = y.y * f[m].y;
         }
-      }
 #pragma unroll
       for (int m = 0; m < 4; ++m) f[m] = lds2(vec + kC * 4 + m * 32);
-      return true;
     };
     bool ok = load_v(0);
     for (int c = 0; ok && c < nchunks; ++c) {
       const int n = c == nchunks - 1 ? tail : kC;
       const uint32_t ph = c & 1;
+      start_chunk(c);
       if (!(ok = wait(&s.d1_full, ph))) break;
       {
         uint32_t d[2][16];
@@ -878,6 +887,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
 
 #pragma unroll
       for (int m = 0; m < 4; ++m) f[m] = lds2(vec + 2 * kC * 4 + m * 32);
+      if (c + 1 < nchunks && !(ok = load_v(c + 1))) break;
       if (!(ok = wait(&s.d3_full, ph))) break;
       {
         uint32_t d[2][16];
@@ -900,15 +910,14 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       hand_over(&s.v_ready);
       decay = lds2(vec + (4 * kC - half * 32 - 2 * t) * 4).x;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) store_tokens(u, kColD1, R[u]);
+      for (int u = 0; u < 2; ++u) store_tokens(u, kColV, R[u]);
       hand_over(&s.p_ready);
-      if (c + 1 < nchunks && !(ok = load_v(c + 1))) break;
 
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         if (!(ok = wait(&s.ds_full[g], ph))) break;
         uint32_t d[32];
-        tmem_ld32(tl + kColDS + g * 64 + half * 32, d);
+        tmem_ld32(tl + kColS + g * 64 + half * 32, d);
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 32; ++j) S[32 * g + j] = fmaf(S[32 * g + j], decay, __uint_as_float(d[j]));
@@ -1048,7 +1057,8 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
     return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
            t.stride(0) > 0 && t.stride(1) > 0;
   };
-  if (T <= kStepMean * R || !rows16(q) || !rows16(k) || !rows16(v) || !rows16(out)) {
+  const int64_t mean = R * HV <= 148 ? kStepMeanOneWave : kStepMean;
+  if (T <= mean * R || !rows16(q) || !rows16(k) || !rows16(v) || !rows16(out)) {
     gdn_step_kernel<<<dim3((unsigned)R, (unsigned)HV), 256, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     return;

@@ -21,9 +21,9 @@ namespace phx {
 
 namespace {
 
-constexpr int kSvThreads = 256;
+constexpr int kSvThreads = 512;
 constexpr int kSvWarps = kSvThreads / 32;
-constexpr int kSvResident = 3;          // CTAs per SM: 85 registers a thread, 16 loads of 16 bytes in flight without spills
+constexpr int kSvResident = 2;          // CTAs per SM: 32 warps, each with three times 16 bytes of both rows a lane in flight
 
 struct SvArgs {
   const void *p, *q;              // q null: greedy drafts
@@ -44,12 +44,6 @@ __device__ __forceinline__ float to_f(T x) {
 
 // weight of index i: max(p - q, 0); NaN gives 0
 __device__ __forceinline__ double weight(float p, float q) { return p > q ? (double)p - (double)q : 0.0; }
-
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 
 // Accepted drafts of request r (warp-wide; every lane gets the count).
 template <typename T>
@@ -73,49 +67,82 @@ __device__ __forceinline__ int accepted(const SvArgs& a, int r, int n, int lane)
   return min(kept, n);
 }
 
-// 16 bytes of a row from element i on, zeros past its end: one load where the row is 16-byte aligned, else element by
-// element.
+// 16 bytes of a row from element i on, zeros past its end. A row that does not start on a 16-byte boundary is read in the
+// two 16-byte granules around them (each holds bytes of the row, so it lies in the row's allocation) and shifted.
 template <typename T>
-__device__ __forceinline__ uint4 load16(const T* row, int i, int V, bool aligned) {
-  constexpr int VEC = 16 / sizeof(T);
-  if (aligned && i + VEC <= V) return *reinterpret_cast<const uint4*>(row + i);
-  using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
-  uint32_t u[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const uint32_t x = i + e < V ? reinterpret_cast<const Bits*>(row)[i + e] : 0;
-    u[e * sizeof(T) / 4] |= x << (8 * (e * sizeof(T) % 4));
+__device__ __forceinline__ uint4 load16(const T* row, int i, int V) {
+  if (i >= V) return make_uint4(0, 0, 0, 0);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + i);
+  const unsigned off = at & 15;
+  const int left = (V - i) * (int)sizeof(T);
+  const uint4* g = reinterpret_cast<const uint4*>(at - off);
+  uint4 u = g[0];
+  if (off) {
+    const uint4 n = left > 16 - (int)off ? g[1] : make_uint4(0, 0, 0, 0);
+    uint64_t w0 = (uint64_t)u.y << 32 | u.x, w1 = (uint64_t)u.w << 32 | u.z, w2 = (uint64_t)n.y << 32 | n.x,
+             w3 = (uint64_t)n.w << 32 | n.z;
+    if (off & 8) w0 = w1, w1 = w2, w2 = w3;
+    const unsigned sh = (off & 7) * 8;
+    if (sh) w0 = w0 >> sh | w1 << (64 - sh), w1 = w1 >> sh | w2 << (64 - sh);
+    u = make_uint4((uint32_t)w0, (uint32_t)(w0 >> 32), (uint32_t)w1, (uint32_t)(w1 >> 32));
   }
-  return make_uint4(u[0], u[1], u[2], u[3]);
+  if (left < 16) {
+    auto keep = [&](uint32_t x, int k) { return left >= 4 * k + 4 ? x : left > 4 * k ? x & 0xffffu : 0u; };
+    u = make_uint4(keep(u.x, 0), keep(u.y, 1), keep(u.z, 2), keep(u.w, 3));
+  }
+  return u;
 }
-template <typename T, int E>
-__device__ __forceinline__ float pick(const uint4& u) {      // element E of 16 bytes
-  const uint32_t w = (E * sizeof(T) / 4) == 0 ? u.x : (E * sizeof(T) / 4) == 1 ? u.y : (E * sizeof(T) / 4) == 2 ? u.z : u.w;
+// element e of 16 bytes (e a constant after unrolling)
+template <typename T>
+__device__ __forceinline__ float pick(const uint4& u, int e) {
+  const int k = e * (int)sizeof(T) / 4;
+  const uint32_t w = k == 0 ? u.x : k == 1 ? u.y : k == 2 ? u.z : u.w;
   if constexpr (sizeof(T) == 4) return __uint_as_float(w);
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w >> (16 * (E & 1)))));
-  else return __uint_as_float((E & 1) ? w & 0xffff0000u : w << 16);
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w >> (16 * (e & 1)))));
+  else return __uint_as_float((e & 1) ? w & 0xffff0000u : w << 16);
+}
+// The part in which the draw falls, of 32 lanes' consecutive parts: the first one with mass whose running sum passes
+// `want`, else (sums in another order may differ in the last bit) the last one with mass, so that an index without mass is
+// never drawn; -1 if none has. `before` grows by the mass of the parts ahead of it. `hit`: whether a sum passed.
+__device__ __forceinline__ int find_part(double part, double& before, double want, int lane, bool& hit) {
+  double upto = part;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += up;
+  }
+  const unsigned some = __ballot_sync(0xffffffffu, part > 0.0), past = __ballot_sync(0xffffffffu, part > 0.0 && before + upto > want);
+  hit = past != 0;
+  if (!some) {
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    return -1;
+  }
+  const int at = past ? __ffs(past) - 1 : 31 - __clz(some);
+  before += __shfl_sync(0xffffffffu, upto - part, at);
+  return at;
 }
 
-constexpr int kSteps = 4;               // 16-byte loads of a row a lane has in flight
-constexpr int kMaxBlocks = 1024;        // block masses a CTA keeps
 constexpr int kMaxCluster = 8;
 
-// A cluster of CTAs (the grid's x) per request. The row is cut into blocks of kSteps x 32 lanes x 16 bytes, `span` times
-// that for rows too long for the table of masses; a CTA takes `blocks` neighbouring ones, a warp every 8th of them. The
-// CTAs exchange their masses through shared memory; the one in which the draw falls finds the block in its table and
-// reads that block again, in order. So the row is read once.
-// Bound: HBM for a full batch on a large vocabulary; else latency (chain values, row, cluster barrier, one block).
-// Measured: see launch().
+// A cluster of CTAs (the grid's x) per request; each warp sums `span` neighbouring steps of 32 lanes x 16 bytes. The CTAs
+// exchange their masses through shared memory. In the one where the draw falls, its warps share the steps of the warp
+// where it falls, which are read a second time (from L2), and the warp that meets it finds the index. So the row comes
+// from memory once, and the sum over a row has no exchange between lanes in it: fp64 additions are far apart.
+// Bound: HBM for a full batch on a large vocabulary; else the chain of dependent reads (token, its probabilities, row,
+// cluster barrier, steps), about 8 us with the launch. Measured (kernel
+// alone, cold cache): 64 requests x 128256 fp32 29 us, 256 x 32000 bf16 17 us, 17 x 32003 bf16 without draft rows 10 us,
+// 1 x 4096 8 us. With 4 x 16 bytes unrolled and a mass per 512 elements: 21 / 17 / 12 / 8, slower over a range of calls.
 template <typename T>
-__global__ void __launch_bounds__(kSvThreads, kSvResident) spec_verify_kernel(const SvArgs a, int blocks, int span) {
+__global__ void __launch_bounds__(kSvThreads, kSvResident) spec_verify_kernel(const SvArgs a, int span) {
   constexpr int VEC = 16 / sizeof(T), kStep = 32 * VEC;
-  __shared__ double mass[kMaxBlocks];
+  __shared__ double mass[2][kSvWarps];
   __shared__ double totals[2][kMaxCluster];
   __shared__ int s_kept;
   const int cl = gridDim.x, rank = blockIdx.x, r = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (cl > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const int n = a.n_draft ? max(0, min(a.D, a.n_draft[r])) : a.D;
+  const float coin = a.coins[(int64_t)r * (a.D + 2) + a.D + 1];
   if (warp == 0) {
     const int k = accepted<T>(a, r, n, lane);
     if (lane == 0) s_kept = k;
@@ -133,65 +160,48 @@ __global__ void __launch_bounds__(kSvThreads, kSvResident) spec_verify_kernel(co
     const int64_t x = a.tokens[(int64_t)r * a.D + kept];
     cut = x >= 0 && x < a.V ? (int)x : -1;
   }
-  const bool p16 = (reinterpret_cast<uintptr_t>(p) & 15) == 0, q16 = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-  const int64_t start = (int64_t)rank * blocks * span * kSteps * kStep;      // this CTA's first element
-  const int nb = (int)min((int64_t)blocks, max((int64_t)0, (a.V - start + span * kSteps * kStep - 1) / (span * kSteps * kStep)));
-  // 16 bytes of each row for each of kSteps steps from element i0 on, and the weights of one step
-  auto load = [&](int64_t i0, uint4 (&x)[kSteps], uint4 (&y)[kSteps]) {
-#pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-      const int i = (int)min(i0 + u * kStep + lane * VEC, (int64_t)a.V);
-      x[u] = load16<T>(p, i, a.V, p16);
-      y[u] = q ? load16<T>(q, i, a.V, q16) : make_uint4(0, 0, 0, 0);
-    }
+  // this lane's first element of a step, its 16 bytes of each row, their weights and their sum
+  const auto first = [&](int step) { return min(step * kStep + lane * VEC, a.V); };     // below 2^31: V is below 2^30
+  const auto load = [&](int i, uint4& x, uint4& y) {
+    x = load16<T>(p, i, a.V);
+    y = q ? load16<T>(q, i, a.V) : make_uint4(0, 0, 0, 0);
   };
-  auto weights = [&](int64_t i0, int u, const uint4& x, const uint4& y, double (&w)[VEC]) {
-    const int64_t i = i0 + u * kStep + lane * VEC;
-    w[0] = weight(pick<T, 0>(x), pick<T, 0>(y)), w[1] = weight(pick<T, 1>(x), pick<T, 1>(y));
-    w[2] = weight(pick<T, 2>(x), pick<T, 2>(y)), w[3] = weight(pick<T, 3>(x), pick<T, 3>(y));
-    if constexpr (VEC == 8) {
-      w[4] = weight(pick<T, 4>(x), pick<T, 4>(y)), w[5] = weight(pick<T, 5>(x), pick<T, 5>(y));
-      w[6] = weight(pick<T, 6>(x), pick<T, 6>(y)), w[7] = weight(pick<T, 7>(x), pick<T, 7>(y));
-    }
-    if (cut >= i && cut < i + VEC) {
+  const auto weights = [&](int i, const uint4& x, const uint4& y, double (&w)[VEC]) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (i + e == cut) w[e] = 0.0;
-    }
+    for (int e = 0; e < VEC; ++e) w[e] = i + e == cut ? 0.0 : weight(pick<T>(x, e), pick<T>(y, e));
+    double m = (w[0] + w[1]) + (w[2] + w[3]);
+    if constexpr (VEC == 8) m += (w[4] + w[5]) + (w[6] + w[7]);
+    return m;
   };
-  const int per = (nb + 31) / 32;         // blocks of a lane's part of the table
-  double total = 0.0, part = 0.0, upto = 0.0;
+  // mass of `count` steps from `step` on, the same in every lane; two loads ahead of the sums
+  const auto steps_mass = [&](int step, int count) {
+    double m = 0.0, w[VEC];
+    uint4 x0, y0, x1, y1;
+    load(count > 0 ? first(step) : a.V, x0, y0);
+    load(count > 1 ? first(step + 1) : a.V, x1, y1);
+#pragma unroll 1
+    for (int k = 0; k < count; ++k) {
+      const uint4 x = x0, y = y0;
+      x0 = x1, y0 = y1;
+      load(k + 2 < count ? first(step + k + 2) : a.V, x1, y1);
+      m += weights(first(step + k), x, y, w);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    return m;
+  };
+  double total = 0.0;
   const double* tot = totals[0];
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     tot = totals[pass];
-    for (int b = warp; b < nb; b += kSvWarps) {
-      double s = 0.0;
-      for (int k = 0; k < span; ++k) {
-        const int64_t i0 = start + ((int64_t)b * span + k) * kSteps * kStep;
-        uint4 x[kSteps], y[kSteps];
-        load(i0, x, y);
-#pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-          double w[VEC];
-          weights(i0, u, x[u], y[u], w);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s += w[e];
-        }
-      }
-      s = warp_sum(s);
-      if (lane == 0) mass[b] = s;
-    }
+    const double m = steps_mass((rank * kSvWarps + warp) * span, span);
+    if (lane == 0) mass[0][warp] = m;
     __syncthreads();
     if (warp == 0) {
-      part = 0.0;
-      for (int b = lane * per; b < min(nb, lane * per + per); ++b) part += mass[b];
-      upto = part;
+      double all = lane < kSvWarps ? mass[0][lane] : 0.0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += up;
-      }
-      const double all = __shfl_sync(0xffffffffu, upto, 31);
+      for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
       if (lane < cl) {
         const uint32_t at = mapa_shared(smem_u32(&totals[pass][rank]), lane);
         asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(all) : "memory");
@@ -200,6 +210,7 @@ __global__ void __launch_bounds__(kSvThreads, kSvResident) spec_verify_kernel(co
     if (cl > 1) cluster_sync();
     else __syncthreads();
     total = 0.0;
+#pragma unroll 1
     for (int c = 0; c < cl; ++c) total += tot[c];
     if (total > 0.0 || (!q && cut < 0)) break;
     // nothing is left of p above q (p = q up to rounding): the draw is from p itself. The second pass exchanges through
@@ -207,89 +218,61 @@ __global__ void __launch_bounds__(kSvThreads, kSvResident) spec_verify_kernel(co
     q = nullptr;
     cut = -1;
   }
-  if (warp != 0) return;
-  // From here on sums in another order than above may differ in the last bit. Only parts with mass are taken, and where
-  // none passes `want` the last one with mass is: an index without mass is never drawn.
-  const double want = (double)a.coins[(int64_t)r * (a.D + 2) + a.D + 1] * total;
+  const double want = (double)coin * total;
   double before = 0.0;
-  int own = 0;
-  for (; own < cl - 1 && !(before + tot[own] > want); ++own) before += tot[own];
-  if (rank != own) return;
-  const unsigned some = __ballot_sync(0xffffffffu, part > 0.0);
-  if (!some) {                            // a row without mass
-    if (lane == 0) a.bonus[r] = a.V - 1;
+  bool hit;
+  const int own = find_part(lane < cl ? tot[lane] : 0.0, before, want, lane, hit);
+  if (own < 0) {                          // a row without mass
+    if (rank == 0 && threadIdx.x == 0) a.bonus[r] = a.V - 1;
     return;
   }
-  const unsigned past = __ballot_sync(0xffffffffu, part > 0.0 && before + upto > want);
-  const int src = past ? __ffs(past) - 1 : 31 - __clz(some);
-  before += __shfl_sync(0xffffffffu, upto - part, src);
-  int block = 0;
-  double skipped = 0.0;
-  for (int b = src * per; b < min(nb, src * per + per); ++b) {   // every lane walks the same few entries
-    if (mass[b] > 0.0) {
-      block = b;
-      skipped = before;
-      if (before + mass[b] > want) break;
-    }
-    before += mass[b];
+  if (rank != own) return;
+  const int ow = max(0, find_part(lane < kSvWarps ? mass[0][lane] : 0.0, before, want, lane, hit));
+  const int sub = (span + kSvWarps - 1) / kSvWarps, base = (rank * kSvWarps + ow) * span;
+  {
+    const double m = steps_mass(base + warp * sub, max(0, min(sub, span - warp * sub)));
+    if (lane == 0) mass[1][warp] = m;
   }
-  before = skipped;
-  int found = -1, last = a.V - 1;
-  for (int k = 0; k < span && found < 0; ++k) {
-    const int64_t i0 = start + ((int64_t)block * span + k) * kSteps * kStep;
-    uint4 x[kSteps], y[kSteps];
-    load(i0, x, y);
+  __syncthreads();
+  const int sw = max(0, find_part(lane < kSvWarps ? mass[1][lane] : 0.0, before, want, lane, hit));
+  if (warp != sw) return;
+  int found = a.V - 1;
+  hit = false;
+#pragma unroll 1
+  for (int k = 0; k < min(sub, span - warp * sub) && !hit; ++k) {
+    const int i = first(base + warp * sub + k);
+    uint4 x, y;
+    load(i, x, y);
+    double w[VEC];
+    const double lsum = weights(i, x, y, w);
+    const int at = find_part(lsum, before, want, lane, hit);
+    if (at < 0) continue;
+    int idx = -1;
+    bool done = false;
+    double acc = before;
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-      if (found >= 0) break;
-      double w[VEC], lsum = 0.0;
-      weights(i0, u, x[u], y[u], w);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) lsum += w[e];
-      double inc = lsum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
+    for (int e = 0; e < VEC; ++e) {
+      if (!done && w[e] > 0.0) {
+        idx = i + e;
+        acc += w[e];
+        done = hit && acc > want;
       }
-      const unsigned any = __ballot_sync(0xffffffffu, lsum > 0.0);
-      const unsigned hit = __ballot_sync(0xffffffffu, lsum > 0.0 && before + inc > want);
-      if (any) {
-        const int at = hit ? __ffs(hit) - 1 : 31 - __clz(any);
-        int idx = -1;
-        if (lane == at) {
-          double acc = before + (inc - lsum);
-          bool done = false;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if (!done && w[e] > 0.0) {
-              idx = (int)(i0 + u * kStep + lane * VEC + e);
-              acc += w[e];
-              done = hit && acc > want;
-            }
-          }
-        }
-        idx = __shfl_sync(0xffffffffu, idx, at);
-        if (hit) found = idx;
-        else last = idx;
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
     }
+    found = __shfl_sync(0xffffffffu, idx, at);
+    before += __shfl_sync(0xffffffffu, lsum, at);
   }
-  if (lane == 0) a.bonus[r] = found >= 0 ? found : last;
+  if (lane == 0) a.bonus[r] = found;
 }
 
 template <typename T>
 void launch(const SvArgs& a, int64_t R, cudaStream_t stream) {
-  constexpr int kBlock = kSteps * 32 * (16 / sizeof(T));
-  const int64_t all = (a.V + kBlock - 1) / kBlock;
-  // CTAs per request: more while the machine's resident CTAs are not all used and a CTA has more blocks than warps (a CTA
-  // with fewer gains nothing, and the cluster's barrier costs about a microsecond)
+  constexpr int kStep = 32 * (16 / sizeof(T));
+  const int64_t steps = (a.V + kStep - 1) / kStep;
+  // CTAs per request: more while all of them are resident at once (a second wave starts its chain of reads anew) and a warp has more than two steps (with
+  // fewer a CTA gains nothing, and the cluster's barrier costs about a microsecond)
   int cl = 1;
-  while (cl < kMaxCluster && R * cl * 2 <= kSvResident * 148 && all > (int64_t)cl * kSvWarps) cl *= 2;
-  int64_t blocks = (all + cl - 1) / cl;
-  const int64_t span = (blocks + kMaxBlocks - 1) / kMaxBlocks;
-  blocks = (blocks + span - 1) / span;
+  while (cl < kMaxCluster && R * cl * 2 <= kSvResident * 148 && steps > (int64_t)cl * 2 * kSvWarps) cl *= 2;
+  const int64_t span = (steps + cl * kSvWarps - 1) / (cl * kSvWarps);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)cl, (unsigned)R);
   cfg.blockDim = dim3(kSvThreads);
@@ -300,7 +283,7 @@ void launch(const SvArgs& a, int64_t R, cudaStream_t stream) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, spec_verify_kernel<T>, a, (int)blocks, (int)span));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, spec_verify_kernel<T>, a, (int)span));
 }
 
 }  // namespace
