@@ -43,8 +43,9 @@ __device__ __forceinline__ bool request(const GdnArgs& a, int r, int& t0, int& t
 
 // Mean tokens per request up to which tokens are taken one by one. Measured, us by steps / by chunks: 1 request x 8 heads,
 // 16 tokens 14.5 / 16.5, 24 tokens 20.6 / 16.5; 64 requests x 16 heads, 8 tokens 58 / 78, 12 tokens 86 / 76; 200 x 32,
-// 4 tokens 331 / 429, 12 tokens 612 / 438: a step costs each wave of CTAs 0.5 us, the chunk form each wave its set-up.
-constexpr int kStepMeanOneWave = 16, kStepMean = 8;
+// 4 tokens 331 / 429, 12 tokens 612 / 438: a step costs each wave of CTAs 0.5 us, the chunk form each wave its set-up of
+// 10 us. All tokens may belong to one request (lengths stay on the device), so steps are also bounded to 64 a wave.
+constexpr int kStepMeanOneWave = 16, kStepMean = 8, kStepsPerWave = 64;
 constexpr int kStepTokens = 16;          // tokens whose q and k are normalised together
 constexpr int kHalf = kDim / 2;
 constexpr int kRowPad = kDim + 8;        // the second half starts 4 floats later: both halves' reads miss each other's banks
@@ -136,8 +137,10 @@ __global__ void __launch_bounds__(256) gdn_step_kernel(const GdnArgs a) {
 //   S1 = e^(b_C) S0 + sum_j e^(b_C - b_j) k^_j v'_j^T
 // gdn_prep_kernel forms X = (I + L)^-1 - I, P and the tokens' factors for every chunk and head at once; gdn_chain_kernel
 // walks the chunks of one (request, head) with the state in registers. The normalisation of k and q is folded into
-// those factors, so the tensor core reads k and q as they are in memory (bf16, exact); every fp32 operand (S, X, P and
-// the two right-hand sides) goes in as two bf16 pieces, hi = bf16(x) and lo = bf16(x - hi), off by at most 2^-18 of x.
+// those factors, so the tensor core reads k and q as they are in memory (bf16, exact). Every fp32 operand goes in as bf16
+// pieces, hi = bf16(x), lo = bf16(x - hi), off by at most 2^-18 of x: S, X, P and V' as two; R and V' c2, whose rounding
+// the state would keep, as three (2^-27). With two for all of them the state after 2048 tokens was off by 2.7e-6 of its
+// norm, of which V' c2 alone made 2.5e-6 and the product of the two lo pieces left out of R^T X^T 1.0e-6; now 0.7e-6.
 // ------------------------------------------------------------------------------------------------
 constexpr int kC = 64;                                   // tokens per chunk
 constexpr int kTri = 5120;                               // one piece of a lower-triangular 64 x 64 matrix, see tri_offset
@@ -160,6 +163,14 @@ __device__ __forceinline__ int first_item(const GdnArgs& a, int r) { return a.to
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(x0, x1);
   lo = pack_bf16x2(x0 - __uint_as_float(hi << 16), x1 - __uint_as_float(hi & 0xffff0000u));
+}
+
+// as split2, and what it leaves
+__device__ __forceinline__ void split3(float x0, float x1, uint32_t& hi, uint32_t& lo, uint32_t& rest) {
+  hi = pack_bf16x2(x0, x1);
+  x0 -= __uint_as_float(hi << 16), x1 -= __uint_as_float(hi & 0xffff0000u);
+  lo = pack_bf16x2(x0, x1);
+  rest = pack_bf16x2(x0 - __uint_as_float(lo << 16), x1 - __uint_as_float(lo & 0xffff0000u));
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -495,12 +506,14 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 //   D4 = V'^T P^T, o = c3 D2 + D4         c3 = e^b scale / |q|
 // The chain's latency bounds it: S -> D1 -> R -> D3 -> V' -> DS -> S. S goes through in two halves of 64 key columns, so
 // that converting one overlaps the products of the other; D2 and the last chunk's D4 run while the state warps work.
-// TMEM columns: DS, then S pieces 128 | D1, then R 64 | D2 64 | D3, then V' c2 pieces 64 | V' pieces 64 | D4 64.
+// TMEM columns: DS, then S pieces 128 | D1, then R 64 | D2 64 | D3, then V' c2 pieces 64 | V' pieces 64 | D4 64 | third
+// pieces of R 32 and of V' c2 32.
 // A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
 // ------------------------------------------------------------------------------------------------
 constexpr int kStages = 3;
 constexpr int kChainThreads = 16 * 32;
-constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColV = 320, kColD4 = 384, kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColD1 = 128, kColD2 = 192, kColD3 = 256, kColV = 320, kColD4 = 384,
+                   kColR3 = 448, kColV3 = 480, kTmemCols = 512;
 constexpr int kStageTx = 3 * kC * kDim * 2 + kItemBytes;
 
 struct ChainStage {
@@ -707,8 +720,8 @@ __global__ void __launch_bounds__(kChainThreads, 1)
         if (elect_one()) umma_f16_ts(tmem + d, hi + 16, db, id64, 1);
       }
     };
-    // D[128 x 64] = A B^T, B lower triangular in two pieces; A in two pieces of 16 columns per 32 tokens
-    auto tri_product = [&](uint32_t d, uint32_t acol, const uint8_t* b) {
+    // D[128 x 64] = A B^T, B lower triangular in two pieces; A in two pieces of 16 columns per 32 tokens, or three
+    auto tri_product = [&](uint32_t d, uint32_t acol, const uint8_t* b, auto third) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         const int rows = kC - 16 * ks;
@@ -718,6 +731,10 @@ __global__ void __launch_bounds__(kChainThreads, 1)
         if (elect_one()) umma_f16_ts(dd, ahi, hi, id, ks > 0);
         if (elect_one()) umma_f16_ts(dd, alo, hi, id, 1);
         if (elect_one()) umma_f16_ts(dd, ahi, lo, id, 1);
+        if constexpr (third.value) {
+          if (elect_one()) umma_f16_ts(dd, alo, lo, id, 1);
+          if (elect_one()) umma_f16_ts(dd, tmem + kColR3 + ks * 8, hi, id, 1);
+        }
       }
     };
     // D[128 x 64] = (V' c2)^T k over the chunk's tokens, key dimensions 64 b .. 64 b + 63 (k MN-major)
@@ -728,12 +745,13 @@ __global__ void __launch_bounds__(kChainThreads, 1)
         const uint32_t ahi = tmem + kColD3 + (ks >> 1) * 32 + (ks & 1) * 8;
         if (elect_one()) umma_f16_ts(tmem + kColS + 64 * b, ahi, db, id64mn, ks > 0);
         if (elect_one()) umma_f16_ts(tmem + kColS + 64 * b, ahi + 16, db, id64mn, 1);
+        if (elect_one()) umma_f16_ts(tmem + kColS + 64 * b, tmem + kColV3 + ks * 8, db, id64mn, 1);
       }
       commit(&s.ds_full[b]);
     };
     auto output_product = [&](int c) {               // D4 of chunk c, the last use of its tiles
       if (!wait(&s.p_ready, c & 1) || (c > 0 && !wait(&s.o_read, (c & 1) ^ 1))) return false;
-      tri_product(kColD4, kColV, s.st[c % kStages].item + 2 * kTri);
+      tri_product(kColD4, kColV, s.st[c % kStages].item + 2 * kTri, std::false_type{});
       commit(&s.o_full);
       commit(&s.empty[c % kStages]);
       return true;
@@ -752,7 +770,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       if (c > 0 && (!output_product(c - 1) || !wait(&s.d2_read, ph ^ 1))) break;
       state_product(kColD2, g.q[0], 0);
       if (!wait(&s.r_ready, ph)) break;
-      tri_product(kColD3, kColD1, g.item);
+      tri_product(kColD3, kColD1, g.item, std::true_type{});
       commit(&s.d3_full);
       state_product(kColD2, g.q[1], 1);
       commit(&s.d2_full);
@@ -797,6 +815,18 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       }
       tmem_st_frag(tl + (u << 20) + col + half * 32, hi);
       tmem_st_frag(tl + (u << 20) + col + half * 32 + 16, lo);
+    };
+    // the same in three pieces, the third at `col3`
+    auto store_tokens3 = [&](int u, uint32_t col, uint32_t col3, const float (&x)[4][4]) {
+      uint32_t hi[8], lo[8], rest[8];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        split3(x[m][0], x[m][1], hi[2 * m], lo[2 * m], rest[2 * m]);
+        split3(x[m][2], x[m][3], hi[2 * m + 1], lo[2 * m + 1], rest[2 * m + 1]);
+      }
+      tmem_st_frag(tl + (u << 20) + col + half * 32, hi);
+      tmem_st_frag(tl + (u << 20) + col + half * 32 + 16, lo);
+      tmem_st_frag(tl + (u << 20) + col3 + half * 16, rest);
     };
     const int t = lane & 3;
     // v tile (token row % 8 = lane % 8, value columns quad * 32 + 8 (lane / 8) ..) of a group of eight tokens
@@ -882,7 +912,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       }
       // every column of this half has been read before its pieces overwrite it
 #pragma unroll
-      for (int u = 0; u < 2; ++u) store_tokens(u, kColD1, R[u]);
+      for (int u = 0; u < 2; ++u) store_tokens3(u, kColD1, kColR3, R[u]);
       hand_over(&s.r_ready);
 
 #pragma unroll
@@ -904,7 +934,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
               R[u][m][e] += __uint_as_float(d[u][4 * m + e]);
               x[m][e] = R[u][m][e] * (e & 1 ? f[m].y : f[m].x);
             }
-          store_tokens(u, kColD3, x);
+          store_tokens3(u, kColD3, kColV3, x);
         }
       }
       hand_over(&s.v_ready);
@@ -1057,8 +1087,8 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
     return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
            t.stride(0) > 0 && t.stride(1) > 0;
   };
-  const int64_t mean = R * HV <= 148 ? kStepMeanOneWave : kStepMean;
-  if (T <= mean * R || !rows16(q) || !rows16(k) || !rows16(v) || !rows16(out)) {
+  const int64_t waves = (R * HV + 147) / 148, mean = waves == 1 ? kStepMeanOneWave : kStepMean;
+  if ((T <= mean * R && T <= kStepsPerWave * waves) || !rows16(q) || !rows16(k) || !rows16(v) || !rows16(out)) {
     gdn_step_kernel<<<dim3((unsigned)R, (unsigned)HV), 256, 0, stream>>>(a);
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     return;

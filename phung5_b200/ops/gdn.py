@@ -69,7 +69,9 @@ def gdn_chunked(q, k, v, g, beta, state, tok_start, slot, scale: float, out: Opt
     """The recurrence of gdn_recurrent(write_state=True) for prompt passes (csrc/gdn_chunk.cu): q, k [T, HK, 128] and
     v [T, HV, 128] bf16 (strided views are taken as they are), g, beta [T, HV] fp32, state [slots, HV, 128, 128] fp32,
     advanced in place at slot[r] over tokens [tok_start[r], tok_start[r + 1]); requests without tokens keep their
-    state. Returns out [T, HV, 128]; rows outside every request are not written."""
+    state, and no two requests share a slot. Slots or token ranges outside their buffers are skipped on the GPU and
+    reported by check_status. Returns out [T, HV, 128]; rows outside every request are not written. g and the state are
+    fp32, kept to about 2^-18 through the chunk products (bf16 pieces of fp32 operands, fp32 sums); out is rounded once."""
     if _check.active():
         _check.gdn_chunked(q, k, v, g, beta, state, tok_start, slot)
     if q.is_cuda:

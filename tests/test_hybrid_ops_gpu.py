@@ -96,7 +96,7 @@ def _gdn_check(a, **kw):
 @pytest.mark.parametrize("lens,hk,hv", [
     ([1], 1, 1), ([2], 4, 8), ([63], 2, 2), ([64], 2, 4), ([65], 1, 4), ([127, 129], 2, 4), ([0, 5, 0], 1, 2),
     ([128, 1, 0, 200, 17], 4, 8), ([1] * 33, 2, 4), ([8] * 20, 4, 8), ([700, 3], 1, 3), ([1500], 16, 32),
-    ([300, 40, 260, 1, 77, 500], 8, 16)])
+    ([300, 40, 260, 1, 77, 500], 8, 16), ([1] * 70 + [400] + [2] * 60, 2, 4), ([3] * 150, 1, 2)])
 def test_gdn_chunked(lens, hk, hv):
     _gdn_check(_gdn_inputs(lens, hk, hv, seed=sum(lens) + hv))
 
@@ -272,7 +272,7 @@ def _qk_check(a, **kw):
     (1, 8, 2, 128, 128, 64, 0), (5, 8, 2, 128, 128, 64, 8), (37, 4, 4, 64, 64, 16, 0), (33, 16, 2, 256, 64, 64, 0),
     (129, 3, 1, 128, 32, 64, 64), (7, 1, 1, 64, 16, 1, 0), (9, 2, 1, 256, 256, 64, 0), (21, 4, 2, 128, 24, 64, 0),
     (6, 2, 2, 80, 80, 64, 0), (6, 3, 1, 96, 22, 64, 0), (4, 2, 1, 10, 6, 8, 0), (3, 2, 1, 512, 512, 64, 0),
-    (17, 4, 2, 128, 128, 64, 3), (2000, 32, 8, 128, 128, 64, 0), (700, 64, 8, 128, 64, 64, 0)])
+    (17, 4, 2, 128, 128, 64, 3), (5, 3, 1, 128, 0, 64, 0), (5, 3, 1, 24, 0, 64, 0), (2000, 32, 8, 128, 128, 64, 0), (700, 64, 8, 128, 64, 64, 0)])
 def test_qk_norm_rope(m, hq, hkv, d, rot, ps, ld):
     _qk_check(_qk_inputs(m, hq, hkv, d, rot, ps, seed=m + d, ld=ld))
 
