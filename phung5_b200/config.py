@@ -52,6 +52,11 @@ class ModelConfig:
     gdn_key_dim: int = 128
     gdn_value_dim: int = 128
     gdn_conv_kernel: int = 4
+    # prompt passes of the GDN layers: "recurrent" (token by token) or "chunked" (64 tokens at a time on the tensor core:
+    # the same recurrence, rounded in other places; 14-23 times as fast on passes of thousands of tokens)
+    gdn_prefill: str = "recurrent"
+    # RMS norm of every query and key head (weights [head_dim] per layer) before the rotation
+    qk_norm: bool = False
 
     @property
     def q_size(self) -> int:
@@ -107,7 +112,9 @@ class SpecConfig:
     accept: "exact" runs the real target-vs-draft acceptance; "geometric" keeps every step of the
     verification (logits, target sampling, acceptance walk) but replaces the accepted length with a
     seeded Geometric(p) draw capped at `accept_cap`, the synthetic-acceptance workload of the
-    benchmark configs (random-init weights never agree with their draft otherwise).
+    benchmark configs (random-init weights never agree with their draft otherwise). "rejection" (chain mode): drafts
+    are sampled from the drafter's distribution under the request's sampling parameters and verified by rejection
+    against it, so that the emitted tokens follow the target's distribution exactly; greedy requests as under "exact".
     """
 
     enabled: bool = True

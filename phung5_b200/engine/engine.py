@@ -96,6 +96,37 @@ class _VocabOps:
         return logits if self.comm.size == 1 else self.comm.all_gather_vocab(logits)
 
 
+class _DraftSampler:
+    """One step's sampled draft chains and their verification by rejection (spec.accept "rejection"): draft d of request
+    r is drawn from the drafter's distribution q_d under the request's temperature, top-k and top-p, and verified against
+    the target's distribution under the same (ops.spec_verify_probs). The drafts' coins come from a hash stream of their
+    own (the request's seed with its bits changed), the verification's from the request's usual one."""
+
+    def __init__(self, eng: "LLMEngine", reqs: List[Request], c: torch.Tensor):
+        self.eng = eng
+        self.temp, self.top_k, self.top_p, seed, _ = eng.sample_tensors(reqs)
+        self.coins = seeded_coins(seed, c, eng.D + 2)
+        self.draft_coins = seeded_coins(seed ^ 0x5EEDD4AF, c, eng.D)
+        self.q: List[torch.Tensor] = []
+
+    def draw(self, logits: torch.Tensor):
+        """Next draft of every request from the drafter's logits -> (scores [R, 1], tokens [R, 1])."""
+        full, d = self.eng.dvocab.full(logits), len(self.q)
+        q = target_probs(full, self.temp, self.top_k, self.top_p)
+        self.q.append(q)
+        R = q.shape[0]
+        coin = torch.stack([torch.zeros_like(self.draft_coins[:, d]), self.draft_coins[:, d]], 1)
+        _, tok = ops.spec_verify_probs(q[:, None], None, torch.empty(R, 0, dtype=torch.int64, device=q.device), coin)
+        return torch.zeros(R, 1, device=q.device), tok[:, None]
+
+    def verify(self, logits: torch.Tensor, tokens: torch.Tensor):
+        """logits [R, D + 1, V_local] of the root and the drafts, tokens [R, D + 1] -> (accepted nodes, bonus)."""
+        R, N = tokens.shape
+        full = self.eng.vocab.full(logits.reshape(R * N, -1))
+        p = target_probs(full, *(t.repeat_interleave(N) for t in (self.temp, self.top_k, self.top_p)))
+        return ops.spec_verify_probs(p.view(R, N, -1), torch.stack(self.q, 1), tokens[:, 1:], self.coins)
+
+
 class _EagerMeta:
     """Attention metadata of the speculative step's forwards, built on the host per forward (page tables
     shared by the step, per-forward lengths and work lists uploaded in one copy each)."""
@@ -126,6 +157,8 @@ class LLMEngine:
         self.dtype = dtype
         mc = cfg.model
         tp = self.comm.size
+        if cfg.spec.enabled and cfg.spec.accept == "rejection" and cfg.spec.mode != "chain":
+            raise ValueError("rejection verifies sampled chains: set spec.mode = 'chain'")
         self.hybrid = mc.arch == "hybrid_gdn"
         gdn_layers = None
         if self.hybrid:
@@ -746,7 +779,7 @@ class LLMEngine:
         return logits, (feat[fb.logits_rows] if feat is not None else None)
 
     def _accept_mode(self, reqs: List[Request]):
-        """("geometric", accept lengths) | ("greedy", None) | ("sample", None)."""
+        """("geometric", accept lengths) | ("greedy", None) | ("sample", None) | ("reject", None)."""
         spec = self.cfg.spec
         if spec.accept == "geometric":
             steps = torch.tensor([r.steps for r in reqs])
@@ -754,14 +787,14 @@ class LLMEngine:
             return "geometric", geometric_accept_len(spec.accept_seed, steps, rid, spec.accept_p, spec.accept_cap)
         if all(r.params.temperature <= 0 for r in reqs):
             return "greedy", None
-        return "sample", None
+        return ("reject" if spec.accept == "rejection" else "sample"), None
 
     def _spec_graph(self, R: int, mode: str, reqs: List[Request]):
         """The CUDA-graph runner for this batch shape and accept mode, or None to run the step eagerly. Seeded
         sampling is captured when the device accept path serves every request."""
         if (self._graphs is None or not self.eagle or self.hybrid
                 or (self.comm.size != 1 and not getattr(self.comm, "fused", False))
-                or (mode == "sample" and not self._device_sampling(reqs))):
+                or mode == "reject" or (mode == "sample" and not self._device_sampling(reqs))):
             return None
         kc = ops.sample_kc([r.params.top_k for r in reqs], [r.params.temperature for r in reqs]) \
             if mode == "sample" else 0
@@ -789,7 +822,8 @@ class LLMEngine:
 
         synth = mode == "geometric" and K > 1
         # ---- tree expansion ----
-        lp, ti = self.dvocab.topk_logprobs(logits, K)          # [R, K]
+        rej = _DraftSampler(self, reqs, c) if mode == "reject" else None     # chains of sampled drafts (K = 1)
+        lp, ti = rej.draw(logits) if rej else self.dvocab.topk_logprobs(logits, K)          # [R, K]
         pool_tok, pool_score = [ti], [lp]
         pool_par = [torch.full((R, K), -1, dtype=torch.int64, device=dev)]
         pool_depth = [torch.ones(R, K, dtype=torch.int64, device=dev)]
@@ -808,7 +842,7 @@ class LLMEngine:
             fb = ForwardBatch(tokens=front_tok.reshape(-1), positions=pos.reshape(-1).to(torch.int32),
                               slots=sl.reshape(-1), meta=dmeta, work1=dw1, work2=dw2)
             lg, fe = self._draft_forward(fb, front_feat.reshape(R * K, -1) if front_feat is not None else None)
-            clp, cti = self.dvocab.topk_logprobs(lg, K)              # [R*K, K]
+            clp, cti = rej.draw(lg) if rej else self.dvocab.topk_logprobs(lg, K)              # [R*K, K]
             cscore = (front_score.reshape(-1, 1) + clp).reshape(R, K * K)
             ctok = cti.reshape(R, K * K)
             cpar = front_idx.reshape(R, K, 1).expand(R, K, K).reshape(R, K * K)
@@ -881,7 +915,9 @@ class LLMEngine:
         self._mark("accept")
         # ---- accept ----
         vl = vlogits.reshape(R, N, -1)
-        if mode == "sample":
+        if rej:
+            acc_nodes, bonus = rej.verify(vl, tokens)
+        elif mode == "sample":
             acc_nodes, bonus = self._accept_sample(reqs, vl, tokens, parent, c, sp)
         else:
             acc_nodes, bonus = self._accept_static(vl, tokens, parent, ngeo)

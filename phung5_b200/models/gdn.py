@@ -36,6 +36,7 @@ class GDNLayer:
     hk: int
     hv: int
     eps: float = 1e-6
+    chunked: bool = False  # prompt passes in chunks (ops.gdn.gdn_chunked) instead of token by token
     _stash: Optional[tuple] = field(default=None, repr=False)
 
     @property
@@ -59,8 +60,11 @@ class GDNLayer:
         k = conv[:, self.hk * 128: 2 * self.hk * 128].reshape(t, self.hk, 128)
         v = conv[:, 2 * self.hk * 128:].reshape(t, self.hv, 128)
         g, beta = G.gdn_gates(a.to(x.dtype), b.to(x.dtype), self.A_log, self.dt_bias)
-        o, st = G.gdn_recurrent(q, k, v, g, beta, state, tok_start, slot, 1.0 / math.sqrt(128),
-                                write_state=not verify, stash=verify)
+        if self.chunked and not verify:
+            o = G.gdn_chunked(q, k, v, g, beta, state, tok_start, slot, 1.0 / math.sqrt(128))
+        else:
+            o, st = G.gdn_recurrent(q, k, v, g, beta, state, tok_start, slot, 1.0 / math.sqrt(128),
+                                    write_state=not verify, stash=verify)
         if verify:
             self._stash = (st, qkv.to(x.dtype), tok_start, slot)
         y = G.gated_rmsnorm(o, z.reshape(t, self.hv, 128).to(o.dtype), self.norm_w, self.eps).reshape(t, -1)

@@ -117,6 +117,8 @@ def random_hybrid(cfg: ModelConfig, device, seed: int = 0, dtype=torch.bfloat16,
     """-> (ModelWeights of the attention layers + embeddings, [GdnLayerWeights or None per layer])."""
     if cfg.quant != "bf16":
         raise ValueError("hybrid GDN models are served in bf16")
+    if cfg.gdn_prefill not in ("recurrent", "chunked"):
+        raise ValueError(f"gdn_prefill {cfg.gdn_prefill!r} is neither 'recurrent' nor 'chunked'")
     full = random_packed_weights(cfg, device, seed=seed)
     attn_layers: List[LayerWeights] = []
     gdn: List[Optional[GdnLayerWeights]] = []
@@ -129,6 +131,7 @@ def random_hybrid(cfg: ModelConfig, device, seed: int = 0, dtype=torch.bfloat16,
         else:
             g = random_gdn_layer(cfg.hidden, hk, hv, device, seed=zlib.crc32(repr((seed, i)).encode()) & 0xFFFF,
                                  conv_w=cfg.gdn_conv_kernel, std=std, dtype=dtype)
+            g.chunked = cfg.gdn_prefill == "chunked"
             gdn.append(GdnLayerWeights(lw.in_norm, lw.post_norm, g, lw.gu, lw.down))
     w = ModelWeights(cfg=cfg, embed=full.embed, layers=attn_layers, final_norm=full.final_norm,
                      lm_head=full.lm_head, vocab_start=full.vocab_start, tp_rank=0, tp_size=1)
@@ -142,7 +145,7 @@ def _cast(w: ModelWeights, dtype) -> ModelWeights:
     def c(t):
         return t.to(dtype) if isinstance(t, torch.Tensor) and t.is_floating_point() else t
     layers = [LayerWeights(c(l.in_norm), c(l.post_norm), Linear(c(l.qkv.w)), Linear(c(l.o.w)), Linear(c(l.gu.w)),
-                           Linear(c(l.down.w))) for l in w.layers]
+                           Linear(c(l.down.w)), q_norm=c(l.q_norm), k_norm=c(l.k_norm)) for l in w.layers]
     return ModelWeights(cfg=w.cfg, embed=c(w.embed), layers=layers, final_norm=c(w.final_norm), lm_head=c(w.lm_head),
                         vocab_start=w.vocab_start, tp_rank=w.tp_rank, tp_size=w.tp_size)
 

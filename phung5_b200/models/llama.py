@@ -8,7 +8,7 @@ rank r keeps heads [r*Hq/tp, (r+1)*Hq/tp) (and the matching KV heads) and FFN co
 Per layer (fp8_block):
   (xq, xs) = add_rmsnorm_quant(h, delta, w_in)       h <- h + delta (previous MLP output, reduced)
   qkv      = gemm_fp8_block(xq, xs, Wqkv)            tcgen05
-  q        = rope_kv_write(qkv, pos, slots)          k/v -> paged cache
+  q        = rope_kv_write(qkv, pos, slots)          k/v -> paged cache (cfg.qk_norm: qk_norm_rope_kv_write)
   (aq, as) = paged_attention(q, ...)                 fp8 output, one scale per (token, head)
   o        = gemm_fp8_block(aq, as, Wo)  -> reduce
   (xq, xs) = add_rmsnorm_quant(h, o, w_post)
@@ -99,6 +99,8 @@ class LayerWeights:
     gu: Optional[Linear] = None       # dense MLP
     down: Optional[Linear] = None
     moe: Optional[object] = None      # MoE block (models/mixtral.py)
+    q_norm: Optional[torch.Tensor] = None   # [head_dim] per-head norm of q and k (cfg.qk_norm)
+    k_norm: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -187,6 +189,9 @@ def pack_weights(cfg: ModelConfig, wd: Dict[str, torch.Tensor], device, tp_rank:
         lw = LayerWeights(in_norm=wd[p + "input_layernorm.weight"].to(device, dtype),
                           post_norm=wd[p + "post_attention_layernorm.weight"].to(device, dtype),
                           qkv=qkv, o=o)
+        if cfg.qk_norm:
+            lw.q_norm = wd[p + "self_attn.q_norm.weight"].to(device, dtype)
+            lw.k_norm = wd[p + "self_attn.k_norm.weight"].to(device, dtype)
         if cfg.is_moe:
             from .mixtral import pack_moe
             lw.moe = pack_moe(cfg, wd, p, device, tp_rank, tp_size, dtype)
@@ -232,6 +237,9 @@ def random_packed_weights(cfg: ModelConfig, device, seed: int = 0, tp_rank: int 
         lw = LayerWeights(in_norm=torch.ones(h, device=device, dtype=torch.bfloat16),
                           post_norm=torch.ones(h, device=device, dtype=torch.bfloat16),
                           qkv=rnd((hq + 2 * hkv) * hd, h, (i, "qkv")), o=rnd(h, hq * hd, (i, "o")))
+        if cfg.qk_norm:
+            lw.q_norm = torch.ones(hd, device=device, dtype=torch.bfloat16)
+            lw.k_norm = torch.ones(hd, device=device, dtype=torch.bfloat16)
         if cfg.is_moe:
             from .mixtral import random_moe
             lw.moe = random_moe(cfg, device, seed, i, tp_rank, tp_size, std)
@@ -331,14 +339,22 @@ class LlamaModel:
                             tiles=tl)
         return out
 
+    def rope(self, li: int, qkv: torch.Tensor, fb: ForwardBatch) -> torch.Tensor:
+        """Rotated (and, with cfg.qk_norm, normed) queries; keys and values go to layer li's cache."""
+        lw, d = self.w.layers[li], self.cfg.head_dim
+        if lw.q_norm is None:
+            return ops.rope_kv_write(qkv, fb.positions, fb.slots, self.cos_sin, self.kv_k[li], self.kv_v[li], self.hq,
+                                     self.hkv, d)
+        return ops.qk_norm_rope_kv_write(qkv, lw.q_norm, lw.k_norm, self.cfg.rms_eps, fb.positions, fb.slots, self.cos_sin,
+                                         self.kv_k[li], self.kv_v[li], self.hq, self.hkv, d)
+
     def layer(self, li: int, h: torch.Tensor, delta: Optional[torch.Tensor], fb: ForwardBatch) -> torch.Tensor:
         lw = self.w.layers[li]
         cfg = self.cfg
         fp8 = lw.qkv.fp8
         xq, xs, xb = ops.add_rmsnorm_quant(h, delta, lw.in_norm, cfg.rms_eps, quant=fp8, out_bf16=not fp8)
         qkv = lw.qkv((xq, xs) if fp8 else xb)
-        q = ops.rope_kv_write(qkv, fb.positions, fb.slots, self.cos_sin, self.kv_k[li], self.kv_v[li], self.hq,
-                              self.hkv, cfg.head_dim)
+        q = self.rope(li, qkv, fb)
         a = self.attention(li, q, fb, fp8)
         o = self.comm.all_reduce(lw.o(a))
         xq, xs, xb = ops.add_rmsnorm_quant(h, o, lw.post_norm, cfg.rms_eps, quant=fp8,
@@ -379,8 +395,7 @@ class LlamaModel:
             _nvtx.push(f"layer{li}")
             lw = self.w.layers[li]
             qkv = lw.qkv(x)
-            q = ops.rope_kv_write(qkv, fb.positions, fb.slots, self.cos_sin, self.kv_k[li], self.kv_v[li], self.hq,
-                                  self.hkv, cfg.head_dim)
+            q = self.rope(li, qkv, fb)
             a = self.attention(li, q, fb, fp8)
             comm.project(lw.o, a, m)
             if lw.moe is not None:

@@ -128,6 +128,9 @@ def decoder_layer(x: torch.Tensor, w: Weights, pre: str, cfg: ModelConfig, posit
     q = (h @ get_weight(w, pre + "self_attn.q_proj.weight").t()).view(t, cfg.num_heads, cfg.head_dim)
     k = (h @ get_weight(w, pre + "self_attn.k_proj.weight").t()).view(t, cfg.num_kv_heads, cfg.head_dim)
     v = (h @ get_weight(w, pre + "self_attn.v_proj.weight").t()).view(t, cfg.num_kv_heads, cfg.head_dim)
+    if pre + "self_attn.q_norm.weight" in w:
+        q = rms_norm(q, w[pre + "self_attn.q_norm.weight"], cfg.rms_eps)
+        k = rms_norm(k, w[pre + "self_attn.k_norm.weight"], cfg.rms_eps)
     q = apply_rope(q, positions, cfg.rope_theta)
     k = apply_rope(k, positions, cfg.rope_theta)
     if len(kv.k) <= li:

@@ -210,11 +210,49 @@ def _checks() -> List[Tuple[str, Callable[[], Tuple[bool, float]]]]:
             ok &= want == got
         return ok, 0.0 if ok else 1.0
 
+    def gdn_chunk():
+        from . import gdn as G
+        t, lens = 205, [70, 1, 134]
+        x = torch.nn.functional.silu(torch.randn(t, 1024, device=dev)).bfloat16()
+        a = dict(q=x[:, :256].view(t, 2, 128), k=x[:, 256:512].view(t, 2, 128), v=x[:, 512:].view(t, 4, 128),
+                 g=-torch.rand(t, 4, device=dev), beta=torch.rand(t, 4, device=dev), state=torch.randn(4, 4, 128, 128, device=dev) * 0.1,
+                 tok_start=torch.tensor([0, 70, 71, 205], dtype=torch.int32, device=dev),
+                 slot=torch.tensor([2, 0, 3], dtype=torch.int32, device=dev), scale=128 ** -0.5)
+        ref = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in a.items()}
+        ref.update({k: ref[k].float() for k in ("q", "k", "v")})
+        o = G.gdn_chunked(**a)
+        e = max(_rel(o, G.gdn_chunked(**ref)) / 4, _rel(a["state"], ref["state"]) * 100)   # one bf16 rounding; fp32
+        return e < 2e-3, e
+
+    def qk_norm_rope():
+        m, hq, hkv, d = 33, 8, 2, 128
+        a = dict(qkv=torch.randn(m, (hq + 2 * hkv) * d, device=dev).bfloat16(), wq=torch.rand(d, device=dev).bfloat16(),
+                 wk=torch.rand(d, device=dev).bfloat16(), eps=1e-6, pos=torch.arange(m, dtype=torch.int32, device=dev),
+                 slots=torch.randperm(128, device=dev)[:m], cos_sin=ops.rope_table(64, 64, 1e6, dev),
+                 k_cache=torch.zeros(2, hkv, 64, d, dtype=torch.bfloat16, device=dev),
+                 v_cache=torch.zeros(2, hkv, 64, d, dtype=torch.bfloat16, device=dev), hq=hq, hkv=hkv, d=d)
+        ref = {k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in a.items()}
+        e = _rel(ops.qk_norm_rope_kv_write(**a), ops.qk_norm_rope_kv_write(**ref))
+        e = max(e, _rel(a["k_cache"], ref["k_cache"]), _rel(a["v_cache"], ref["v_cache"]))
+        return e < 2e-3, e
+
+    def spec_verify():
+        R, D, V = 9, 4, 5003
+        x = torch.randn(R, D + 1, V, device=dev) * 3
+        p = torch.softmax(x, -1)
+        q = torch.softmax(x[:, :D] + 0.5 * torch.randn(R, D, V, device=dev), -1)
+        tok, coins = q.argmax(-1), torch.rand(R, D + 2, device=dev).clamp_(max=0.999)
+        got = ops.spec_verify_probs(p, q, tok, coins)
+        want = ops.spec_verify_probs(p.cpu(), q.cpu(), tok.cpu(), coins.cpu())
+        ok = all(torch.equal(g.cpu(), w) for g, w in zip(got, want))
+        return ok, 0.0 if ok else 1.0
+
     return [("gemm_fp8_block", gemm_fp8), ("gemm_bf16", gemm_bf16), ("gemm_grouped", gemm_grouped),
             ("gemm_split_k", gemm_split), ("add_rmsnorm_quant", norm_quant), ("silu_mul_quant", silu_quant),
             ("topk_logprobs", topk), ("argmax", argmax), ("paged_attention", attention), ("raster", raster),
             ("gemm_fp8_swiglu", gemm_swiglu), ("moe_combine", moe_combine), ("rope_kv_write", rope_kv),
-            ("gdn_recurrent", gdn_verify), ("sample_candidates", sample_candidates)]
+            ("gdn_recurrent", gdn_verify), ("sample_candidates", sample_candidates),
+            ("gdn_chunked", gdn_chunk), ("qk_norm_rope_kv_write", qk_norm_rope), ("spec_verify_probs", spec_verify)]
 
 
 def run() -> Dict[str, dict]:

@@ -45,6 +45,9 @@ def random_weights(cfg: ModelConfig, seed: int = 0, std: float = 0.02, device="c
         for nm, n in (("q_proj", cfg.q_size), ("k_proj", cfg.kv_size), ("v_proj", cfg.kv_size)):
             _add_linear(w, p + f"self_attn.{nm}.weight", _linear(g, n, h, std, device).to(dtype), fp8)
         _add_linear(w, p + "self_attn.o_proj.weight", _linear(g, h, cfg.q_size, std, device).to(dtype), fp8)
+        if cfg.qk_norm:
+            for nm in ("q_norm", "k_norm"):
+                w[p + f"self_attn.{nm}.weight"] = torch.ones(cfg.head_dim, device=device, dtype=dtype)
         if cfg.is_moe:
             w[p + "block_sparse_moe.gate.weight"] = _linear(g, cfg.num_experts, h, std, device).to(dtype)
             for e in range(cfg.num_experts):

@@ -26,6 +26,7 @@ docker/opt/prefetch/prefetch_shim.sh:24-35); this loader reads such a directory 
 """
 from __future__ import annotations
 
+import dataclasses
 import json
 import os
 from typing import Dict, Iterator, Mapping, Optional, Tuple
@@ -142,7 +143,10 @@ def load_config(path: str) -> ModelConfig:
 
 
 def open_checkpoint(path: str) -> Tuple[ModelConfig, Checkpoint]:
-    return load_config(path), Checkpoint(path)
+    mc, ck = load_config(path), Checkpoint(path)
+    if "model.layers.0.self_attn.q_norm.weight" in ck:     # per-head q/k norms: told by their weights
+        mc = dataclasses.replace(mc, qk_norm=True)
+    return mc, ck
 
 
 def load_model(path: str, device, tp_rank: int = 0, tp_size: int = 1, cfg: Optional[ModelConfig] = None):
