@@ -232,6 +232,9 @@ struct PrepSmem {
 };
 __host__ __device__ constexpr int blk_of(int bi, int bj) { return bi * (bi + 1) / 2 + bj; }
 
+// Bound: instruction issue (7500 warp instructions an item and head, half of them ALU; DRAM at a fifth). Measured: 9728
+// items x heads in 140 us, 1024 in 25 us (one head a CTA; 96 instead of 128 registers: 145 and 30). Forward substitution of
+// all 64 rows by one thread a column took 330 us: 2600 unrolled instructions, fetched anew by every CTA.
 // One CTA per (work item, `heads` value heads of one key head). The Gram matrices come from mma.sync and stay in its
 // registers; each head's P and factors go from there to memory (a warp's 4-byte stores fill 128 bytes). (I + L)^-1 by
 // blocks of 16: the diagonal ones by forward substitution, one column per thread, then 16 -> 32 -> 64 by
@@ -240,6 +243,8 @@ __host__ __device__ constexpr int blk_of(int bi, int bj) { return bi * (bi + 1) 
 __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8_t* __restrict__ items, int heads) {
   __shared__ __align__(128) PrepSmem s;
   const int w = blockIdx.x, hk = blockIdx.y * heads / (a.HV / a.HK);
+  // the chain's CTAs may take the SMs that this grid leaves; they wait for its end before they read an item
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int lo = 0, hi = a.R - 1;            // the last request whose items start at or before w
   while (lo < hi) {
@@ -309,18 +314,25 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
     }
   }
 
+  // a head's gates and betas: tokens 2 l and 2 l + 1 in lane l of warp 0 and of warp 1, loaded a head ahead
+  float in0 = 0.f, in1 = 0.f;
+  auto fetch = [&](int h) {
+    const float* src = warp == 0 ? a.g : a.beta;
+    if (warp < 2) {
+      in0 = 2 * lane < n ? src[(int64_t)(t0 + 2 * lane) * a.HV + h] : 0.f;
+      in1 = 2 * lane + 1 < n ? src[(int64_t)(t0 + 2 * lane + 1) * a.HV + h] : 0.f;
+    }
+  };
+  fetch(blockIdx.y * heads);
   for (int hh = 0; hh < heads; ++hh) {
     const int h = blockIdx.y * heads + hh;
     uint8_t* item = items + ((int64_t)w * a.HV + h) * kItemBytes;
     // ---- the head's sums of g and betas ----
     if (warp == 0) {
       // e^-1e6 is 0 as e^-inf is, and its sums can be subtracted
-      auto gate = [&](int i) -> double {
-        const float x = i < n ? a.g[(int64_t)(t0 + i) * a.HV + h] : 0.f;
-        return x < -1e6f ? -1e6f : x;
-      };
-      double b0 = gate(2 * lane);
-      const double b1 = b0 + gate(2 * lane + 1);
+      auto gate = [](float x) -> double { return x < -1e6f ? -1e6f : x; };
+      double b0 = gate(in0);
+      const double b1 = b0 + gate(in1);
       double inc = b1;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -332,10 +344,10 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
       inc *= kLog2e;
       s.bh[2 * lane] = (float)b0, s.bl[2 * lane] = (float)(b0 - (float)b0);
       s.bh[2 * lane + 1] = (float)inc, s.bl[2 * lane + 1] = (float)(inc - (float)inc);
-    } else if (warp < 3) {
-      const int i = tid - 32;
-      s.beta[i] = i < n ? a.beta[(int64_t)(t0 + i) * a.HV + h] : 0.f;
+    } else if (warp == 1) {
+      s.beta[2 * lane] = in0, s.beta[2 * lane + 1] = in1;
     }
+    if (hh + 1 < heads) fetch(h + 1);
     __syncthreads();     // the blocks take the place of k and q (or of the last head's blocks); the factors are complete
     float* vec = reinterpret_cast<float*>(item + 4 * kTri);
     if (tid < kC) {
@@ -509,6 +521,10 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 // TMEM columns: DS, then S pieces 128 | D1, then R 64 | D2 64 | D3, then V' c2 pieces 64 | V' pieces 64 | D4 64 | third
 // pieces of R 32 and of V' c2 32.
 // A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
+// Measured: 2.57 us a chunk (128 chunks of 8 heads in 329 us), 2.2 of them before R and V' c2 got their third pieces; the
+// tensor core is busy for 1.2 us of it (a product with A in TMEM costs N / 2 cycles), the state warps' conversions for 1.
+// One waiting lane at the issuer, all waits with a timer, one lane per value column in every token: 3.9 us. Requests in
+// order of length, the longest first: 250 instead of 260 us for 48 requests of 16384 tokens, lost again on ordering them.
 // ------------------------------------------------------------------------------------------------
 constexpr int kStages = 3;
 constexpr int kChainThreads = 16 * 32;
@@ -633,7 +649,10 @@ __global__ void __launch_bounds__(kChainThreads, 1)
   const int warp = warp_id(), lane = lane_id();
   const int r = blockIdx.y, h = blockIdx.x, hk = h / (a.HV / a.HK);
   int t0, t1, slot;
-  if (!request(a, r, t0, t1, slot) || t0 == t1) return;   // uniform, before any barrier or TMEM use
+  if (!request(a, r, t0, t1, slot) || t0 == t1) {         // uniform, before any barrier or TMEM use
+    asm volatile("griddepcontrol.wait;" ::: "memory");    // what follows in the stream follows the first kernel too
+    return;
+  }
   const int nchunks = (t1 - t0 + kC - 1) / kC;
   const int tail = t1 - t0 - (nchunks - 1) * kC;           // tokens of the last chunk
 
@@ -664,6 +683,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
   if (warp == 0) {
     // ---------------- loader ----------------
     const int item0 = first_item(a, r);
+    asm volatile("griddepcontrol.wait;" ::: "memory");      // the items are complete
     int issued = 0;
     bool ok = true;
     for (int c = 0; c < nchunks; ++c) {
@@ -1115,8 +1135,20 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   const int rep = (int)(HV / HK), heads = n_items * HK >= 4 * 148 ? rep : 1;
   gdn_prep_kernel<<<dim3((unsigned)n_items, (unsigned)(HV / heads)), 128, 0, stream>>>(a, it, heads);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  gdn_chain_kernel<<<dim3((unsigned)HV, (unsigned)R), kChainThreads, chain_smem, stream>>>(tk, tq, tv, to, a, it);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  // The chain starts while the items are still being made: its set-up and first loads of the state need none. Everything
+  // before the two kernels is complete by then (the first one is launched in order), and every CTA of the first has
+  // started before one of the second takes an SM.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)HV, (unsigned)R);
+  cfg.blockDim = dim3(kChainThreads);
+  cfg.dynamicSmemBytes = chain_smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, gdn_chain_kernel, tk, tq, tv, to, a, (const uint8_t*)it));
 }
 
 }  // namespace phx

@@ -53,7 +53,7 @@ class ModelConfig:
     gdn_value_dim: int = 128
     gdn_conv_kernel: int = 4
     # prompt passes of the GDN layers: "recurrent" (token by token) or "chunked" (64 tokens at a time on the tensor core:
-    # the same recurrence, rounded in other places; 14-23 times as fast on passes of thousands of tokens)
+    # the same recurrence, rounded in other places; 12 to 18 times as fast on passes of thousands of tokens)
     gdn_prefill: str = "recurrent"
     # RMS norm of every query and key head (weights [head_dim] per layer) before the rotation
     qk_norm: bool = False
