@@ -1103,9 +1103,10 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
             (int)T, (int)R, (int)HK, (int)HV, (int)state.size(0), (float)scale};
   const at::cuda::CUDAGuard guard(q.device());
   auto stream = at::cuda::getCurrentCUDAStream();
-  auto rows16 = [](const torch::Tensor& t) {   // what 16-byte loads and tensor maps need
-    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
-           t.stride(0) > 0 && t.stride(1) > 0;
+  auto head_stride = [](const torch::Tensor& t) { return t.size(1) == 1 ? kDim : t.stride(1); };   // one head: any stride
+  auto rows16 = [&](const torch::Tensor& t) {   // what 16-byte loads and tensor maps need
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % 8 == 0 && head_stride(t) % 8 == 0 &&
+           t.stride(0) > 0 && head_stride(t) > 0;
   };
   const int64_t waves = (R * HV + 147) / 148, mean = waves == 1 ? kStepMeanOneWave : kStepMean;
   if ((T <= mean * R && T <= kStepsPerWave * waves) || !rows16(q) || !rows16(k) || !rows16(v) || !rows16(out)) {
@@ -1117,7 +1118,7 @@ void gdn_chunked(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   const int64_t n_items = T / kC + R;
   torch::Tensor items = torch::empty({n_items * HV * kItemBytes}, q.options().dtype(at::kByte));
   auto map = [&](const torch::Tensor& t, int64_t heads) {
-    return make_tmap_3d(t.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kDim, heads, T, t.stride(1) * 2, t.stride(0) * 2, 64, 1, kC,
+    return make_tmap_3d(t.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kDim, heads, T, head_stride(t) * 2, t.stride(0) * 2, 64, 1, kC,
                         CU_TENSOR_MAP_SWIZZLE_128B);
   };
   const CUtensorMap tk = map(k, HK), tq = map(q, HK), tv = map(v, HV), to = map(out, HV);

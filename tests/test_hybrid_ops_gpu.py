@@ -101,6 +101,21 @@ def test_gdn_chunked(lens, hk, hv):
     _gdn_check(_gdn_inputs(lens, hk, hv, seed=sum(lens) + hv))
 
 
+@pytest.mark.parametrize("lens", [[200, 3, 66], [5, 9]])
+def test_gdn_chunked_any_layout(lens):
+    """Rows off 16-byte boundaries, heads apart, one head with a stride of its own, an output of the caller's."""
+    a = _gdn_inputs(lens, 2, 4, seed=11)
+    ref = _gdn_check({**a, "state": a["state"].clone()})
+    t = sum(lens)
+    off = {k: torch.empty(a[k].numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view(a[k].shape).copy_(a[k]) for k in ("q", "k", "v")}
+    _gdn_check({**a, **off, "state": a["state"].clone()})
+    wide = {k: torch.zeros(t, a[k].shape[1], 200, dtype=torch.bfloat16, device=DEV)[..., :128].copy_(a[k]) for k in ("q", "k", "v")}
+    assert torch.equal(_gdn_check({**a, **wide, "state": a["state"].clone()}, out=torch.empty_like(ref)), ref)
+    b = _gdn_inputs(lens, 1, 1, seed=12)
+    one = {k: torch.as_strided(b[k].contiguous(), (t, 1, 128), (128, 1, 1)) for k in ("q", "k", "v")}
+    _gdn_check({**b, **one})
+
+
 @pytest.mark.parametrize("kind", ["no decay", "hard decay", "resets", "one key", "zeros", "large"])
 @pytest.mark.parametrize("lens", [[200, 70], [5, 1, 9]])
 def test_gdn_chunked_values(kind, lens):
