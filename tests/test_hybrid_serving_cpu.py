@@ -121,3 +121,15 @@ def test_hybrid_rejection_runs_with_everything_on():
 
     a, b, mixed, greedy = run((0.8, 0.8)), run((0.8, 0.8)), run((0.8, 0.0)), run((0.0, 0.0))
     assert a == b and mixed == [a[0], greedy[1]] and a != greedy
+
+
+def test_bounds_checks_pass_on_a_whole_run():
+    """Every index that the engine hands to these operators passes the bounds-check mode, and it changes no token."""
+    from phung5_b200.ops import check
+    cfg = preset("tiny-hybrid", qk_norm=True, gdn_prefill="chunked")
+    prompts, sp = [[1, 2, 3, 4, 5] * 6, [7, 8, 9]], SamplingParams(max_new_tokens=6, temperature=0.8, top_k=20, seed=3)
+    ref = _engine(cfg, temperature_mode="rejection").generate(prompts, sp)
+    with check.bounds_checks():
+        before = check.CHECKS[0]
+        assert _engine(cfg, temperature_mode="rejection").generate(prompts, sp) == ref
+        assert check.CHECKS[0] > before
