@@ -208,6 +208,42 @@ def case_gdn_verify(reqs, n, hk, hv):
     return fn, reqs * hv * 128 * 128 * 4 + t * (2 * hk + hv) * 128 * 2 + t * hv * 128 * (2 + 8), "bytes"
 
 
+def case_gdn_chunked(reqs, n, hk, hv):
+    from ..ops import gdn as G
+    t = reqs * n
+    x = torch.nn.functional.silu(torch.randn(t, (2 * hk + hv) * 128, device="cuda")).bfloat16()
+    q, k, v = (s.view(t, -1, 128) for s in x.split([hk * 128, hk * 128, hv * 128], 1))
+    g, beta = -torch.rand(t, hv, device="cuda") * 0.1, torch.rand(t, hv, device="cuda")
+    state = torch.zeros(reqs, hv, 128, 128, device="cuda")
+    ts = torch.arange(reqs + 1, device="cuda", dtype=torch.int32) * n
+    slot = torch.arange(reqs, device="cuda", dtype=torch.int32)
+    fn = lambda: G.gdn_chunked(q, k, v, g, beta, state, ts, slot, 128 ** -0.5)
+    # q/k/v/gates read and out written once, state in and out
+    return fn, t * ((2 * hk + 2 * hv) * 256 + 8 * hv) + reqs * 2 * hv * 128 * 128 * 4, "bytes"
+
+
+def case_qk_norm_rope(m, hq, hkv):
+    from .. import ops
+    d = 128
+    qkv = torch.randn(m, (hq + 2 * hkv) * d, device="cuda").bfloat16()
+    w = torch.ones(d, device="cuda", dtype=torch.bfloat16)
+    cs = ops.rope_table(8192, d, 5e5, "cuda")
+    kc = torch.zeros((m + 63) // 64, hkv, 64, d, device="cuda", dtype=torch.bfloat16)
+    vc = torch.zeros_like(kc)
+    pos, slots = torch.arange(m, device="cuda", dtype=torch.int32), torch.arange(m, device="cuda")
+    fn = lambda: ops.qk_norm_rope_kv_write(qkv, w, w, 1e-6, pos, slots, cs, kc, vc, hq, hkv, d)
+    return fn, m * ((hq + 2 * hkv) * d * 4 + d * 4 + 12), "bytes"
+
+
+def case_spec_verify_probs(reqs, drafts, v):
+    from .. import ops
+    x = torch.randn(reqs, drafts + 1, v, device="cuda") * 3
+    p, q = torch.softmax(x, -1), torch.softmax(x[:, :drafts] + 0.4 * torch.randn(reqs, drafts, v, device="cuda"), -1)
+    tok, coins = q.argmax(-1), torch.rand(reqs, drafts + 2, device="cuda").clamp_(max=0.999)
+    fn = lambda: ops.spec_verify_probs(p, q, tok, coins)
+    return fn, reqs * 2 * v * 4, "bytes"       # one row of both per request
+
+
 def case_raster(ntri, size):
     from ..render import scene as S
     g = torch.Generator().manual_seed(0)
@@ -319,6 +355,9 @@ CASES = {
     "add_rmsnorm_quant": lambda: case_rmsnorm_quant(4096, 8192),
     "rope_kv_write": lambda: case_rope_kv(4096, 64, 8),
     "gdn_verify_64x8": lambda: case_gdn_verify(64, 8, 16, 32),
+    "gdn_chunked_8x1024": lambda: case_gdn_chunked(8, 1024, 16, 32),
+    "qk_norm_rope_kv_write": lambda: case_qk_norm_rope(4096, 64, 8),
+    "spec_verify_probs_64x4": lambda: case_spec_verify_probs(64, 4, 128256),
     "raster_100k_512": lambda: case_raster(100_000, 512),
     "topk8_draft_tp8": lambda: case_topk(512, 16032, 8),
     "topk8_draft": lambda: case_topk(512, 128256, 8),
