@@ -50,14 +50,17 @@ constexpr int kStepTokens = 16;          // tokens whose q and k are normalised 
 constexpr int kHalf = kDim / 2;
 constexpr int kRowPad = kDim + 8;        // the second half starts 4 floats later: both halves' reads miss each other's banks
 
-__global__ void __launch_bounds__(256) gdn_step_kernel(const GdnArgs a) {
-  __shared__ __align__(16) float sq[kStepTokens][kRowPad], sk[kStepTokens][kRowPad];
-  __shared__ float sdec[kStepTokens], sbeta[kStepTokens];
-  const int h = blockIdx.y, hk = h / (a.HV / a.HK);
-  int t0, t1, slot;
-  if (!request(a, blockIdx.x, t0, t1, slot) || t0 == t1) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int j = threadIdx.x >> 1, half = threadIdx.x & 1;
+struct StepSmem {
+  float q[kStepTokens][kRowPad], k[kStepTokens][kRowPad];
+  float dec[kStepTokens], beta[kStepTokens];
+};
+
+// Tokens [t0, t1) of one request and value head, by 256 threads; `sync` joins them.
+template <class Sync>
+__device__ __forceinline__ void step_tokens(const GdnArgs& a, int h, int t0, int t1, int slot, int tid, StepSmem& s, Sync sync) {
+  const int hk = h / (a.HV / a.HK);
+  const int warp = tid >> 5, lane = tid & 31;
+  const int j = tid >> 1, half = tid & 1;
   const int hoff = half * (kHalf + 4);
   float* S = a.state + ((int64_t)slot * a.HV + h) * kDim * kDim + half * kHalf * kDim + j;
   float col[kHalf];
@@ -85,49 +88,56 @@ __global__ void __launch_bounds__(256) gdn_step_kernel(const GdnArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = lane + 32 * e, pi = i < kHalf ? i : i + 4;
-        sq[u][pi] = qv[e] * qn;
-        sk[u][pi] = kv[e] * kn;
+        s.q[u][pi] = qv[e] * qn;
+        s.k[u][pi] = kv[e] * kn;
       }
       if (lane == 0) {
-        sdec[u] = expf(a.g[(int64_t)(c0 + u) * a.HV + h]);
-        sbeta[u] = a.beta[(int64_t)(c0 + u) * a.HV + h];
+        s.dec[u] = expf(a.g[(int64_t)(c0 + u) * a.HV + h]);
+        s.beta[u] = a.beta[(int64_t)(c0 + u) * a.HV + h];
       }
     }
-    __syncthreads();
+    sync();
     for (int u = 0; u < n; ++u) {
       const float vj = __bfloat162float(a.v[(int64_t)(c0 + u) * a.v_t + h * a.v_h + j]);
-      const float decay = sdec[u];
-      const float4* k4 = reinterpret_cast<const float4*>(&sk[u][hoff]);
-      const float4* q4 = reinterpret_cast<const float4*>(&sq[u][hoff]);
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float decay = s.dec[u];
+      const float4* k4 = reinterpret_cast<const float4*>(&s.k[u][hoff]);
+      const float4* q4 = reinterpret_cast<const float4*>(&s.q[u][hoff]);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < kHalf / 4; ++i) {
         const float4 kk = k4[i];
-        s.x = fmaf(col[4 * i] *= decay, kk.x, s.x);
-        s.y = fmaf(col[4 * i + 1] *= decay, kk.y, s.y);
-        s.z = fmaf(col[4 * i + 2] *= decay, kk.z, s.z);
-        s.w = fmaf(col[4 * i + 3] *= decay, kk.w, s.w);
+        sum.x = fmaf(col[4 * i] *= decay, kk.x, sum.x);
+        sum.y = fmaf(col[4 * i + 1] *= decay, kk.y, sum.y);
+        sum.z = fmaf(col[4 * i + 2] *= decay, kk.z, sum.z);
+        sum.w = fmaf(col[4 * i + 3] *= decay, kk.w, sum.w);
       }
-      float kv = (s.x + s.y) + (s.z + s.w);
+      float kv = (sum.x + sum.y) + (sum.z + sum.w);
       kv += __shfl_xor_sync(0xffffffffu, kv, 1);
-      const float vp = (vj - kv) * sbeta[u];
-      s = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float vp = (vj - kv) * s.beta[u];
+      sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < kHalf / 4; ++i) {
         const float4 kk = k4[i], qq = q4[i];
-        s.x = fmaf(col[4 * i] = fmaf(kk.x, vp, col[4 * i]), qq.x, s.x);
-        s.y = fmaf(col[4 * i + 1] = fmaf(kk.y, vp, col[4 * i + 1]), qq.y, s.y);
-        s.z = fmaf(col[4 * i + 2] = fmaf(kk.z, vp, col[4 * i + 2]), qq.z, s.z);
-        s.w = fmaf(col[4 * i + 3] = fmaf(kk.w, vp, col[4 * i + 3]), qq.w, s.w);
+        sum.x = fmaf(col[4 * i] = fmaf(kk.x, vp, col[4 * i]), qq.x, sum.x);
+        sum.y = fmaf(col[4 * i + 1] = fmaf(kk.y, vp, col[4 * i + 1]), qq.y, sum.y);
+        sum.z = fmaf(col[4 * i + 2] = fmaf(kk.z, vp, col[4 * i + 2]), qq.z, sum.z);
+        sum.w = fmaf(col[4 * i + 3] = fmaf(kk.w, vp, col[4 * i + 3]), qq.w, sum.w);
       }
-      float o = (s.x + s.y) + (s.z + s.w);
+      float o = (sum.x + sum.y) + (sum.z + sum.w);
       o += __shfl_xor_sync(0xffffffffu, o, 1);
       if (half == 0) a.out[((int64_t)(c0 + u) * a.HV + h) * kDim + j] = __float2bfloat16(o);
     }
-    __syncthreads();   // the next tokens rewrite the shared rows
+    sync();   // the next tokens rewrite the shared rows
   }
 #pragma unroll
   for (int i = 0; i < kHalf; ++i) S[i * kDim] = col[i];
+}
+
+__global__ void __launch_bounds__(256) gdn_step_kernel(const GdnArgs a) {
+  __shared__ __align__(16) StepSmem s;
+  int t0, t1, slot;
+  if (!request(a, blockIdx.x, t0, t1, slot) || t0 == t1) return;
+  step_tokens(a, blockIdx.y, t0, t1, slot, threadIdx.x, s, [] { __syncthreads(); });
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -521,6 +531,11 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 // TMEM columns: DS, then S pieces 128 | D1, then R 64 | D2 64 | D3, then V' c2 pieces 64 | V' pieces 64 | D4 64 | third
 // pieces of R 32 and of V' c2 32.
 // A later product overwrites what an earlier one read: the tensor core runs one thread's products in order.
+// The products multiply whole blocks of a chunk, zeros above the diagonals among them, and 0 * NaN is NaN: a NaN, an
+// infinity or an overflow in one token would reach tokens ahead of it, which the recurrence leaves alone. Whatever is not
+// finite in k, v, g, beta, X or S makes V' so, and through it the state, which stays so: if an element of the last state
+// is not finite, the state warps take the request's tokens one by one from the state in memory, which is written only at
+// the end. A q that is not finite reaches its own token's outputs alone.
 // Measured: 2.57 us a chunk (128 chunks of 8 heads in 329 us), 2.2 of them before R and V' c2 got their third pieces; the
 // tensor core is busy for 1.2 us of it (a product with A in TMEM costs N / 2 cycles), the state warps' conversions for 1.
 // One waiting lane at the issuer, all waits with a timer, one lane per value column in every token: 3.9 us. Requests in
@@ -546,6 +561,7 @@ struct ChainSmem {
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
+  int redo;                      // an element of the new state is not finite
 };
 
 // MN-major SWIZZLE_128B operand: `lbo` bytes between 64-element blocks along N, 1024 between 8-row groups along K.
@@ -665,7 +681,7 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     for (uint64_t* b : {&s.s_ready[0], &s.s_ready[1], &s.r_ready, &s.v_ready, &s.p_ready}) mbar_init(b, 8);
     for (uint64_t* b : {&s.d2_read, &s.o_read, &s.o_staged}) mbar_init(b, 4);
     for (uint64_t* b : {&s.d1_full, &s.d2_full, &s.d3_full, &s.ds_full[0], &s.ds_full[1], &s.o_full, &s.mma_done}) mbar_init(b, 1);
-    s.abort = 0;
+    s.abort = s.redo = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -978,12 +994,22 @@ __global__ void __launch_bounds__(kChainThreads, 1)
       }
       if (!ok) break;
     }
-    if (!ok) {
-      give_up(status, kErrTimeoutEpilogue, abort);
-    } else {
+    if (!ok) give_up(status, kErrTimeoutEpilogue, abort);
+    float odd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 64; ++j) odd[j & 3] = fmaf(S[j], 0.f, odd[j & 3]);       // NaN if one is not finite
+    if ((odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.f) *static_cast<volatile int*>(&s.redo) = 1;
+    asm volatile("bar.sync 1, 256;" ::: "memory");      // every state warp has looked
+    const bool redo = *static_cast<volatile int*>(&s.redo);
+    if (ok && !redo) {
 #pragma unroll
       for (int j = 0; j < 64; ++j) gS[((j >> 5) * 64 + (j & 31)) * kDim] = S[j];
     }
+    asm volatile("bar.sync 2, 384;" ::: "memory");      // the outputs are in memory; who gave up has said so
+    // the stages' memory is free: every copy has landed and every product and store from it is complete
+    if (__builtin_expect(redo && !*abort, 0))
+      step_tokens(a, h, t0, t1, slot, threadIdx.x - 128, *reinterpret_cast<StepSmem*>(s.st),
+                  [] { asm volatile("bar.sync 3, 256;" ::: "memory"); });
   } else if (warp >= 12) {
     // ---------------- output warps ----------------
     regs_down<112>();
@@ -1066,6 +1092,8 @@ __global__ void __launch_bounds__(kChainThreads, 1)
     }
     if (c < nchunks) give_up(status, kErrTimeoutEpilogue, abort);
     if (warp == 12 && lane == 0) bulk_wait0();
+    __syncwarp();
+    asm volatile("bar.sync 2, 384;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();

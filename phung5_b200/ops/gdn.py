@@ -71,7 +71,9 @@ def gdn_chunked(q, k, v, g, beta, state, tok_start, slot, scale: float, out: Opt
     advanced in place at slot[r] over tokens [tok_start[r], tok_start[r + 1]); requests without tokens keep their
     state, and no two requests share a slot. Slots or token ranges outside their buffers are skipped on the GPU and
     reported by check_status. Returns out [T, HV, 128]; rows outside every request are not written. g and the state are
-    fp32, kept to about 2^-18 through the chunk products (bf16 pieces of fp32 operands, fp32 sums); out is rounded once."""
+    fp32, kept to about 2^-18 through the chunk products (bf16 pieces of fp32 operands, fp32 sums); out is rounded once.
+    A value that is not finite reaches what it reaches in the recurrence, never an earlier token: a (request, head) whose
+    new state is not finite is taken again token by token (half a microsecond a token)."""
     if _check.active():
         _check.gdn_chunked(q, k, v, g, beta, state, tok_start, slot)
     if q.is_cuda:
