@@ -65,6 +65,18 @@ def gdn_recurrent(q, k, v, g, beta, state, tok_start, slot, scale: float, write_
     return out, st
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    if a.numel() == 0 or b.numel() == 0 or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+
+    def span(x):
+        lo = x.storage_offset() * x.element_size()
+        return lo, lo + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def gdn_chunked(q, k, v, g, beta, state, tok_start, slot, scale: float, out: Optional[torch.Tensor] = None):
     """The recurrence of gdn_recurrent(write_state=True) for prompt passes (csrc/gdn_chunk.cu): q, k [T, HK, 128] and
     v [T, HV, 128] bf16 (strided views are taken as they are), g, beta [T, HV] fp32, state [slots, HV, 128, 128] fp32,
@@ -73,7 +85,10 @@ def gdn_chunked(q, k, v, g, beta, state, tok_start, slot, scale: float, out: Opt
     reported by check_status. Returns out [T, HV, 128]; rows outside every request are not written. g and the state are
     fp32, kept to about 2^-18 through the chunk products (bf16 pieces of fp32 operands, fp32 sums); out is rounded once.
     A value that is not finite reaches what it reaches in the recurrence, never an earlier token: a (request, head) whose
-    new state is not finite is taken again token by token (half a microsecond a token)."""
+    new state is not finite is taken again token by token (half a microsecond a token). `out` shares no memory with q, k,
+    v, g or beta."""
+    if out is not None and any(_share_memory(out, x) for x in (q, k, v, g, beta)):
+        raise ValueError("gdn_chunked: out shares memory with an input")
     if _check.active():
         _check.gdn_chunked(q, k, v, g, beta, state, tok_start, slot)
     if q.is_cuda:
