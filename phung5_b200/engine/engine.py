@@ -102,19 +102,40 @@ class _DraftSampler:
     the target's distribution under the same (ops.spec_verify_probs). The drafts' coins come from a hash stream of their
     own (the request's seed with its bits changed), the verification's from the request's usual one."""
 
+    # Probabilities formed at a time: the dense definition (engine/sampling.py) holds up to 64 bytes of sorted values,
+    # indices and sums for each, so 0.5 GiB beside the two results, whatever the batch.
+    PIECE = 1 << 23
+
     def __init__(self, eng: "LLMEngine", reqs: List[Request], c: torch.Tensor):
         self.eng = eng
         self.temp, self.top_k, self.top_p, seed, _ = eng.sample_tensors(reqs)
         self.coins = seeded_coins(seed, c, eng.D + 2)
         self.draft_coins = seeded_coins(seed ^ 0x5EEDD4AF, c, eng.D)
-        self.q: List[torch.Tensor] = []
+        self.q: Optional[torch.Tensor] = None        # [R, D, V]
+        self.drawn = 0
+
+    def _probs(self, vocab: _VocabOps, logits: torch.Tensor, per: int) -> torch.Tensor:
+        """logits [R * per, V_local] -> the requests' distributions [R * per, V] fp32."""
+        params = [t.repeat_interleave(per) for t in (self.temp, self.top_k, self.top_p)]
+        n, step = logits.shape[0], max(1, self.PIECE // self.eng.cfg.model.vocab)      # the same on every rank
+        out = None
+        for a in range(0, n, step):
+            p = target_probs(vocab.full(logits[a:a + step]), *(t[a:a + step] for t in params))
+            if n <= step:
+                return p
+            if out is None:
+                out = p.new_empty(n, p.shape[1])
+            out[a:a + step] = p
+        return out
 
     def draw(self, logits: torch.Tensor):
         """Next draft of every request from the drafter's logits -> (scores [R, 1], tokens [R, 1])."""
-        full, d = self.eng.dvocab.full(logits), len(self.q)
-        q = target_probs(full, self.temp, self.top_k, self.top_p)
-        self.q.append(q)
+        q, d = self._probs(self.eng.dvocab, logits, 1), self.drawn
         R = q.shape[0]
+        if self.q is None:
+            self.q = q.new_empty(R, self.eng.D, q.shape[1])
+        self.q[:, d] = q
+        self.drawn += 1
         coin = torch.stack([torch.zeros_like(self.draft_coins[:, d]), self.draft_coins[:, d]], 1)
         _, tok = ops.spec_verify_probs(q[:, None], None, torch.empty(R, 0, dtype=torch.int64, device=q.device), coin)
         return torch.zeros(R, 1, device=q.device), tok[:, None]
@@ -122,9 +143,8 @@ class _DraftSampler:
     def verify(self, logits: torch.Tensor, tokens: torch.Tensor):
         """logits [R, D + 1, V_local] of the root and the drafts, tokens [R, D + 1] -> (accepted nodes, bonus)."""
         R, N = tokens.shape
-        full = self.eng.vocab.full(logits.reshape(R * N, -1))
-        p = target_probs(full, *(t.repeat_interleave(N) for t in (self.temp, self.top_k, self.top_p)))
-        return ops.spec_verify_probs(p.view(R, N, -1), torch.stack(self.q, 1), tokens[:, 1:], self.coins)
+        p = self._probs(self.eng.vocab, logits.reshape(R * N, -1), N)
+        return ops.spec_verify_probs(p.view(R, N, -1), self.q, tokens[:, 1:], self.coins)
 
 
 class _EagerMeta:
@@ -810,7 +830,8 @@ class LLMEngine:
 
     def _spec_core(self, mp, pt, c, roots, logits, root_feat, mode, ngeo, reqs=None, sp=None):
         """Tree expansion, selection, verification, acceptance and the KV move of one speculative step, on
-        device tensors only (no host synchronisation unless mode == "sample" takes the dense torch definition).
+        device tensors only (no host synchronisation unless the dense torch definition of the distributions is taken:
+        mode "reject", and mode "sample" where a request needs it).
         `sp`: sampling tensors (mode "sample"; None: uploaded from reqs). `mp` supplies the attention
         metadata and work lists of the draft rounds and of verification. Returns packed [R, 2 + D] int64:
         accepted count, accepted tokens (-1 padded), bonus token."""

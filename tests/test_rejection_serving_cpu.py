@@ -1,0 +1,49 @@
+"""Sampled draft chains verified by rejection, through the engine and its sampler (CPU)."""
+from types import SimpleNamespace
+
+import torch
+
+from phung5_b200 import ops
+from phung5_b200.engine import engine as E
+from phung5_b200.engine.sampling import seeded_coins, target_probs
+
+
+def _sampler(R, D, V, temps=None, top_k=0, top_p=1.0):
+    """A _DraftSampler over a stand-in engine with whole vocabularies."""
+    temps = torch.full((R,), 0.8) if temps is None else temps
+    vocab = SimpleNamespace(full=lambda x: x)
+    eng = SimpleNamespace(D=D, vocab=vocab, dvocab=vocab, cfg=SimpleNamespace(model=SimpleNamespace(vocab=V)),
+                          sample_tensors=lambda reqs: (temps, torch.full((R,), top_k, dtype=torch.int32), torch.full((R,), top_p),
+                                                       torch.arange(R) + 5, None))
+    return E._DraftSampler(eng, [None] * R, torch.arange(R) + 11)
+
+
+def test_dense_distributions_are_formed_in_bounded_pieces(monkeypatch):
+    """64 requests x 5 drafts of a large vocabulary: no call of the dense definition takes more than 2^23 probabilities,
+    and the step is the one that the whole tensors give."""
+    R, D, V = 64, 5, 32003
+    g = torch.Generator().manual_seed(3)
+    dl = [torch.randn(R, V, generator=g) * 2 for _ in range(D)]
+    vl = torch.randn(R, D + 1, V, generator=g) * 2
+    for d in range(D):
+        vl[:, d] = 0.9 * dl[d] + 0.2 * vl[:, d]               # near enough that drafts are kept
+    sizes = []
+
+    def spy(logits, *args):
+        sizes.append(logits.numel())
+        return target_probs(logits, *args)
+    monkeypatch.setattr(E, "target_probs", spy)
+    s = _sampler(R, D, V, top_k=50, top_p=0.95)
+    drafts = [s.draw(x)[1] for x in dl]
+    tokens = torch.cat([torch.zeros(R, 1, dtype=torch.int64)] + drafts, 1)
+    acc, bonus = s.verify(vl, tokens)
+    assert max(sizes) <= 1 << 23
+    par = (torch.full((R,), 0.8), torch.full((R,), 50), torch.full((R,), 0.95))
+    q = torch.stack([target_probs(x, *par) for x in dl], 1)
+    p = torch.stack([target_probs(vl[:, d], *par) for d in range(D + 1)], 1)
+    ra, rb = ops.spec_verify_probs(p, q, tokens[:, 1:], seeded_coins(torch.arange(R) + 5, torch.arange(R) + 11, D + 2))
+    assert torch.equal(acc, ra) and torch.equal(bonus, rb)
+    n = (acc >= 0).sum(1)
+    assert 0 < int(n.sum()) < R * D
+    for d, x in enumerate(drafts):
+        assert bool((q[:, d].gather(1, x) > 0).all())
