@@ -110,7 +110,8 @@ class _DraftSampler:
         self.eng = eng
         self.temp, self.top_k, self.top_p, seed, _ = eng.sample_tensors(reqs)
         self.coins = seeded_coins(seed, c, eng.D + 2)
-        self.draft_coins = seeded_coins(seed ^ 0x5EEDD4AF, c, eng.D)
+        # a chain without drafts takes the root's draw too (its node is not verified)
+        self.draft_coins = seeded_coins(seed ^ 0x5EEDD4AF, c, max(eng.D, 1))
         self.q: Optional[torch.Tensor] = None        # [R, D, V]
         self.drawn = 0
 
@@ -134,7 +135,8 @@ class _DraftSampler:
         R = q.shape[0]
         if self.q is None:
             self.q = q.new_empty(R, self.eng.D, q.shape[1])
-        self.q[:, d] = q
+        if d < self.eng.D:
+            self.q[:, d] = q
         self.drawn += 1
         coin = torch.stack([torch.zeros_like(self.draft_coins[:, d]), self.draft_coins[:, d]], 1)
         _, tok = ops.spec_verify_probs(q[:, None], None, torch.empty(R, 0, dtype=torch.int64, device=q.device), coin)

@@ -1,11 +1,16 @@
 """Sampled draft chains verified by rejection, through the engine and its sampler (CPU)."""
 from types import SimpleNamespace
 
+import pytest
 import torch
 
 from phung5_b200 import ops
+from phung5_b200.config import CacheConfig, DraftConfig, EngineConfig, SpecConfig, preset
 from phung5_b200.engine import engine as E
+from phung5_b200.engine.oracle import SamplingParams
 from phung5_b200.engine.sampling import seeded_coins, target_probs
+from phung5_b200.models.llama import pack_weights
+from phung5_b200.weights.init import random_weights
 
 
 def _sampler(R, D, V, temps=None, top_k=0, top_p=1.0):
@@ -47,3 +52,18 @@ def test_dense_distributions_are_formed_in_bounded_pieces(monkeypatch):
     assert 0 < int(n.sum()) < R * D
     for d, x in enumerate(drafts):
         assert bool((q[:, d].gather(1, x) > 0).all())
+
+
+def _engine(accept, num_draft=2, model=None, drafter=None, **kw):
+    return E.LLMEngine(EngineConfig(model=model or preset("tiny"), spec=SpecConfig(mode="chain", num_draft=num_draft, accept=accept),
+                                    draft=DraftConfig(kind="model", num_layers=1), cache=CacheConfig(page_size=16, num_pages=128), **kw),
+                       device="cpu", dtype=torch.float32, max_context=256, drafter=drafter)
+
+
+def test_chains_without_drafts():
+    """num_draft 0 emits one token a step, drawn from the target's distribution, under every accept rule."""
+    eng = _engine("rejection", num_draft=0)
+    outs = eng.generate([[1, 2, 3], [4, 5]], SamplingParams(max_new_tokens=5, temperature=0.8, seed=1))
+    assert [len(o) for o in outs] == [5, 5] and all(a == 0 for r in eng.reqs.values() for a in r.accepted)
+    again = _engine("rejection", num_draft=0).generate([[1, 2, 3], [4, 5]], SamplingParams(max_new_tokens=5, temperature=0.8, seed=1))
+    assert again == outs
