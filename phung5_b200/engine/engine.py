@@ -179,6 +179,8 @@ class LLMEngine:
         self.dtype = dtype
         mc = cfg.model
         tp = self.comm.size
+        if cfg.spec.enabled and cfg.spec.accept not in ("exact", "geometric", "rejection"):
+            raise ValueError(f"spec.accept {cfg.spec.accept!r} is neither 'exact', 'geometric' nor 'rejection'")
         if cfg.spec.enabled and cfg.spec.accept == "rejection" and cfg.spec.mode != "chain":
             raise ValueError("rejection verifies sampled chains: set spec.mode = 'chain'")
         self.hybrid = mc.arch == "hybrid_gdn"

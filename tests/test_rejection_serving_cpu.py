@@ -67,3 +67,15 @@ def test_chains_without_drafts():
     assert [len(o) for o in outs] == [5, 5] and all(a == 0 for r in eng.reqs.values() for a in r.accepted)
     again = _engine("rejection", num_draft=0).generate([[1, 2, 3], [4, 5]], SamplingParams(max_new_tokens=5, temperature=0.8, seed=1))
     assert again == outs
+
+
+@pytest.mark.parametrize("accept", ["reject", "Rejection", "", "greedy"])
+def test_unknown_accept_rules_are_refused(accept):
+    with pytest.raises(ValueError, match="accept"):
+        _engine(accept)
+
+
+def test_accept_is_not_read_without_speculation():
+    cfg = EngineConfig(model=preset("tiny"), spec=SpecConfig(enabled=False, accept="none"), cache=CacheConfig(page_size=16, num_pages=64))
+    eng = E.LLMEngine(cfg, device="cpu", dtype=torch.float32, max_context=256)
+    assert len(eng.generate([[1, 2]], SamplingParams(max_new_tokens=3))[0]) == 3
