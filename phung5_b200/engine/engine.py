@@ -241,6 +241,9 @@ class LLMEngine:
                         **{**mc.to_dict(), "num_layers": cfg.draft.num_layers,
                            "arch": "llama" if mc.arch == "hybrid_gdn" else mc.arch})
                     dw = random_packed_weights(dcfg, self.device, seed=cfg.seed + 1, tp_rank=self.comm.rank, tp_size=tp)
+                if spec.accept == "rejection" and dw.lm_head.shape[0] != target.lm_head.shape[0]:
+                    raise ValueError(f"rejection compares distributions over one vocabulary: the drafter has {dw.lm_head.shape[0]} "
+                                     f"tokens, the target {target.lm_head.shape[0]}")
                 self.drafter = LlamaModel(dw, self.pool.dk, self.pool.dv, self.cos_sin, self.comm)
         self.vocab = _VocabOps(self.comm, target.vocab_start)
         self.dvocab = _VocabOps(self.comm, self.drafter.w.vocab_start if (self.drafter is not None and not self.eagle)
