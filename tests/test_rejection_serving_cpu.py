@@ -1,4 +1,5 @@
 """Sampled draft chains verified by rejection, through the engine and its sampler (CPU)."""
+import dataclasses
 from types import SimpleNamespace
 
 import pytest
@@ -10,6 +11,7 @@ from phung5_b200.engine import engine as E
 from phung5_b200.engine.oracle import SamplingParams
 from phung5_b200.engine.sampling import seeded_coins, target_probs
 from phung5_b200.models.llama import pack_weights
+from phung5_b200.models.reference import RefModel
 from phung5_b200.weights.init import random_weights
 
 
@@ -91,3 +93,37 @@ def test_rejection_needs_a_drafter_of_the_targets_vocabulary():
     same = pack_weights(cfg, random_weights(cfg, seed=2, std=0.05), "cpu", dtype=torch.float32)
     out = _engine("rejection", model=cfg, drafter=same).generate([[1, 2, 3]], SamplingParams(max_new_tokens=6, temperature=0.7, seed=2))
     assert len(out[0]) == 6
+
+
+def test_the_drafts_of_a_chain_are_drawn_independently():
+    """The second token after the root given the first, over 4000 seeds, against the target's distribution: drafts that
+    share a coin would make it follow from the first. A frequency of n draws is off by more than 4.5 standard deviations (of
+    at most 0.5 / sqrt(n)) about once in 10^5; some 300 frequencies are looked at."""
+    cfg = dataclasses.replace(preset("tiny"), name="eight-tokens", num_layers=1, hidden=64, num_heads=2, num_kv_heads=2, head_dim=32,
+                              ffn=96, vocab=8)
+    w = random_weights(cfg, seed=7, std=0.3)
+    g = torch.Generator().manual_seed(4)
+    near = {k: v + 0.05 * torch.randn(v.shape, generator=g) if v.dim() == 2 else v for k, v in w.items()}
+    pack = lambda x: pack_weights(cfg, x, "cpu", dtype=torch.float32)  # noqa: E731
+    prompt, n = [3, 1, 4, 1, 5], 4000
+    eng = E.LLMEngine(EngineConfig(model=cfg, spec=SpecConfig(mode="chain", num_draft=2, accept="rejection"), max_running=1024,
+                                   draft=DraftConfig(kind="model", num_layers=1), cache=CacheConfig(page_size=16, num_pages=4096)),
+                      device="cpu", dtype=torch.float32, max_context=256, target=pack(w), drafter=pack(near))
+    rids = [eng.add_request(prompt, SamplingParams(max_new_tokens=3, temperature=1.0, seed=s)) for s in range(n)]
+    while eng.has_work():
+        eng.step()
+    outs = [eng.reqs[r].out for r in rids]
+    first = [eng.reqs[r].accepted[0] for r in rids]
+    assert sum(a == 2 for a in first) > n // 4 and first.count(0) > n // 50       # both drafts kept, and rejections
+    ref, seen = RefModel(cfg, w), 0
+    for a in range(8):
+        for b in range(8):
+            group = [o[2] for o in outs if o[:2] == [a, b]]
+            if len(group) < 100:
+                continue
+            logits, _ = ref.forward(torch.tensor(prompt + [a, b]), torch.arange(7), ref.new_cache())
+            p = target_probs(logits[-1:], torch.ones(1), torch.zeros(1, dtype=torch.int64), torch.ones(1))[0]
+            freq = torch.bincount(torch.tensor(group), minlength=8) / len(group)
+            assert (freq - p).abs().max() < 4.5 * 0.5 / len(group) ** 0.5
+            seen += 1
+    assert seen >= 8
