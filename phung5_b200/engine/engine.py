@@ -245,6 +245,7 @@ class LLMEngine:
                     raise ValueError(f"rejection compares distributions over one vocabulary: the drafter has {dw.lm_head.shape[0]} "
                                      f"tokens, the target {target.lm_head.shape[0]}")
                 self.drafter = LlamaModel(dw, self.pool.dk, self.pool.dv, self.cos_sin, self.comm)
+        self._status = ops.StatusReader(self.device)
         self.vocab = _VocabOps(self.comm, target.vocab_start)
         self.dvocab = _VocabOps(self.comm, self.drafter.w.vocab_start if (self.drafter is not None and not self.eagle)
                                 else target.vocab_start)
@@ -503,6 +504,28 @@ class LLMEngine:
         self.pool.prefix.release(r.pages)
         r.pages = []
 
+    def _check_device(self, reqs: List[Request]) -> None:
+        """After a wait that followed `_status.fetch()`: raise if a kernel has reported an error since the last step.
+        The word does not tell whose tokens, KV pages or recurrent states it spoilt, so every request in flight (`reqs`:
+        the step's own) is dropped with its pages, and the cached prefixes go too; requests that had not started stay
+        queued."""
+        try:
+            self._status.check()
+        except RuntimeError:
+            for r in reqs + self.running + self.waiting:
+                if r.finished or (not r.pages and r.gslot < 0):
+                    continue
+                if r.gslot >= 0:
+                    self.gdn_pool.release(r.gslot)
+                    r.gslot = -1
+                self.pool.prefix.release(r.pages)
+                r.pages = []
+                r.finished, r.finish_reason, r.t_done = True, "abort", time.perf_counter()
+            self.running = []
+            self.waiting = [r for r in self.waiting if not r.finished]
+            self.pool.prefix.evict(len(self.pool.prefix.lru))
+            raise
+
     def _emit(self, r: Request, new: List[int]) -> StepOutput:
         room = r.params.max_new_tokens - len(r.out)
         new = new[:room]
@@ -646,7 +669,9 @@ class LLMEngine:
             self.running.append(r)
         done = [(i, r) for i, r in done if all(r is not x for x in resumed)]
         if done:
+            self.stats["d2h_bytes"] += self._status.fetch()
             firsts = self._first_token(logits[[i for i, _ in done]], [r for _, r in done])
+            self._check_device([r for r, _, _ in batch])
             for (i, r), t in zip(done, firsts):
                 r.root = t
                 r.tokens.append(t)
@@ -672,8 +697,10 @@ class LLMEngine:
         if self.hybrid:
             fb.gdn = self._gdn_batch([1] * len(reqs), reqs, "prefill")
         logits, _ = self.target.forward(fb)
+        self.stats["d2h_bytes"] += self._status.fetch()
         nxt = self._first_token(logits, reqs) if any(r.params.temperature > 0 for r in reqs) else \
             self.vocab.argmax(logits).tolist()
+        self._check_device(reqs)
         outs = []
         for r, t in zip(reqs, nxt):
             r.committed += 1
@@ -763,7 +790,9 @@ class LLMEngine:
                                          mode, ngeo, reqs)
 
         self._mark("commit_sync")
+        self.stats["d2h_bytes"] += self._status.fetch()
         packed = packed_dev.cpu()
+        self._check_device(reqs)
         self.stats["d2h_bytes"] += packed.numel() * packed.element_size()
         outs = []
         for i, r in enumerate(reqs):

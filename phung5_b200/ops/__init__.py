@@ -6,7 +6,8 @@ definition of the op, which is also the oracle the GPU tests compare against and
 suite exercises (engine logic, multi-rank gloo runs).
 
 Kernel status: kernels with bounded waits write a nonzero code into a per-device int32 status word
-instead of hanging; `check_status()` raises if any kernel reported a timeout.
+instead of hanging; `check_status()` raises if any kernel reported a timeout or another error (the engine reads
+the same word every step).
 """
 from __future__ import annotations
 
@@ -130,10 +131,32 @@ def check_status(device=None) -> None:
     devs = [torch.device(device)] if device is not None else [torch.device("cuda", i) for i in _STATUS]
     for d in devs:
         t = status_tensor(d)
-        v = int(t[0].item())
-        if v:
-            t.zero_()
-            raise RuntimeError(f"kernel status on {d}: {STATUS_CODES.get(v, v)}")
+        _raise_status(int(t[0].item()), t)
+
+
+def _raise_status(v: int, t: torch.Tensor) -> None:
+    if v:
+        t.zero_()
+        raise RuntimeError(f"kernel status on {t.device}: {STATUS_CODES.get(v, v)}")
+
+
+class StatusReader:
+    """check_status without a wait of its own, for callers that wait for the device anyway: `fetch` copies the word to
+    the host in stream order and returns the bytes copied, `check`, after the caller's wait, raises as check_status does."""
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True) if self.device.type == "cuda" else None
+
+    def fetch(self) -> int:
+        if self.host is None:
+            return 0
+        self.host.copy_(status_tensor(self.device)[:1], non_blocking=True)
+        return 4
+
+    def check(self) -> None:
+        if self.host is not None:
+            _raise_status(int(self.host[0]), status_tensor(self.device))
 
 
 # ------------------------------------------------------------------------------------------------
