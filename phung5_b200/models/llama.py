@@ -192,6 +192,9 @@ def pack_weights(cfg: ModelConfig, wd: Dict[str, torch.Tensor], device, tp_rank:
         if cfg.qk_norm:
             lw.q_norm = wd[p + "self_attn.q_norm.weight"].to(device, dtype)
             lw.k_norm = wd[p + "self_attn.k_norm.weight"].to(device, dtype)
+            for name, t in (("q_norm", lw.q_norm), ("k_norm", lw.k_norm)):
+                if t.numel() != cfg.head_dim:
+                    raise ValueError(f"{p}self_attn.{name}.weight has {t.numel()} elements: norms are taken per head ({cfg.head_dim})")
         if cfg.is_moe:
             from .mixtral import pack_moe
             lw.moe = pack_moe(cfg, wd, p, device, tp_rank, tp_size, dtype)
