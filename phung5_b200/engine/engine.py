@@ -109,6 +109,7 @@ class _DraftSampler:
     def __init__(self, eng: "LLMEngine", reqs: List[Request], c: torch.Tensor):
         self.eng = eng
         self.temp, self.top_k, self.top_p, seed, _ = eng.sample_tensors(reqs)
+        self.greedy = bool((self.temp <= 0).any())       # the step's one wait of its own
         self.coins = seeded_coins(seed, c, eng.D + 2)
         # a chain without drafts takes the root's draw too (its node is not verified)
         self.draft_coins = seeded_coins(seed ^ 0x5EEDD4AF, c, max(eng.D, 1))
@@ -117,11 +118,11 @@ class _DraftSampler:
 
     def _probs(self, vocab: _VocabOps, logits: torch.Tensor, per: int) -> torch.Tensor:
         """logits [R * per, V_local] -> the requests' distributions [R * per, V] fp32."""
-        params = [t.repeat_interleave(per) for t in (self.temp, self.top_k, self.top_p)]
+        params = [t.repeat_interleave(per) if per > 1 else t for t in (self.temp, self.top_k, self.top_p)]
         n, step = logits.shape[0], max(1, self.PIECE // self.eng.cfg.model.vocab)      # the same on every rank
         out = None
         for a in range(0, n, step):
-            p = target_probs(vocab.full(logits[a:a + step]), *(t[a:a + step] for t in params))
+            p = target_probs(vocab.full(logits[a:a + step]), *(t[a:a + step] for t in params), self.greedy)
             if n <= step:
                 return p
             if out is None:
@@ -866,8 +867,8 @@ class LLMEngine:
 
     def _spec_core(self, mp, pt, c, roots, logits, root_feat, mode, ngeo, reqs=None, sp=None):
         """Tree expansion, selection, verification, acceptance and the KV move of one speculative step, on
-        device tensors only (no host synchronisation unless the dense torch definition of the distributions is taken:
-        mode "reject", and mode "sample" where a request needs it).
+        device tensors only (no host synchronisation in modes "geometric" and "greedy", nor in mode "sample" unless it takes
+        the dense torch definition; mode "reject" waits once).
         `sp`: sampling tensors (mode "sample"; None: uploaded from reqs). `mp` supplies the attention
         metadata and work lists of the draft rounds and of verification. Returns packed [R, 2 + D] int64:
         accepted count, accepted tokens (-1 padded), bonus token."""

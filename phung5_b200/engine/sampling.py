@@ -64,12 +64,13 @@ def seeded_coins(seed: torch.Tensor, prefix_len: torch.Tensor, ncols: int) -> to
 
 
 def target_probs(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
-                 top_p: torch.Tensor) -> torch.Tensor:
+                 top_p: torch.Tensor, any_greedy: Optional[bool] = None) -> torch.Tensor:
     """logits [R, V] (any float), per-row temperature/top_k/top_p [R] -> probs [R, V] fp32.
 
     Temperature divides with IEEE division (the reference's topkbf kernel uses div.rn.f32,
     docker/opt/v5/topkbf_normcfg/topkbf/kopt_topkbf.py:134-141). top_k <= 0 means no top-k cut;
-    top_p >= 1 means no nucleus cut. Rows with temperature 0 become one-hot at the argmax."""
+    top_p >= 1 means no nucleus cut. Rows with temperature 0 become one-hot at the argmax (any_greedy: whether there
+    are any; None: looked up, which waits for the device)."""
     x = logits.float()
     greedy = temperature <= 0
     t = torch.where(greedy, torch.ones_like(temperature), temperature).float()
@@ -88,7 +89,7 @@ def target_probs(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
     sp = sp * keep_p
     sp = sp / sp.sum(-1, keepdim=True)
     probs = torch.zeros_like(x).scatter_(-1, si, sp)
-    if greedy.any():
+    if greedy.any() if any_greedy is None else any_greedy:
         onehot = torch.zeros_like(x).scatter_(-1, logits.float().argmax(-1, keepdim=True), 1.0)
         probs = torch.where(greedy[:, None], onehot, probs)
     return probs
