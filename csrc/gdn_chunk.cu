@@ -44,7 +44,8 @@ __device__ __forceinline__ bool request(const GdnArgs& a, int r, int& t0, int& t
 // Mean tokens per request up to which tokens are taken one by one. Measured, us by steps / by chunks: 1 request x 8 heads,
 // 16 tokens 14.5 / 16.5, 24 tokens 20.6 / 16.5; 64 requests x 16 heads, 8 tokens 58 / 78, 12 tokens 86 / 76; 200 x 32,
 // 4 tokens 331 / 429, 12 tokens 612 / 438: a step costs each wave of CTAs 0.5 us, the chunk form each wave its set-up of
-// 10 us. All tokens may belong to one request (lengths stay on the device), so steps are also bounded to 64 a wave.
+// 10 us. All tokens may belong to one request (lengths stay on the device), so steps are also bounded to 64 a wave, except
+// where q, k, v or out are off the boundaries that the chunk form's copies need: those calls have no other form.
 constexpr int kStepMeanOneWave = 16, kStepMean = 8, kStepsPerWave = 64;
 constexpr int kStepTokens = 16;          // tokens whose q and k are normalised together
 constexpr int kHalf = kDim / 2;

@@ -83,7 +83,12 @@ def gdn_chunked(q, k, v, g, beta, state, tok_start, slot, scale: float, out: Opt
     advanced in place at slot[r] over tokens [tok_start[r], tok_start[r + 1]); requests without tokens keep their
     state, and no two requests share a slot. Slots or token ranges outside their buffers are skipped on the GPU and
     reported by check_status. Returns out [T, HV, 128]; rows outside every request are not written. g and the state are
-    fp32, kept to about 2^-18 through the chunk products (bf16 pieces of fp32 operands, fp32 sums); out is rounded once.
+    fp32; out is rounded once. In the chunk form fp32 operands enter the tensor core as two or three bf16 pieces with fp32
+    sums: one is off by at most 2^-18 of itself, states measured within 1e-6 of their norm.
+    The form goes by the batch: chunks where its requests have more than 8 tokens in the mean (16 where all heads run at
+    once), token by token below, so that a request's last bits depend on what it is batched with. The tensor core needs q,
+    k, v and out on 16-byte boundaries (base, and token and head strides of multiples of 8 elements above 0): a call
+    with one that is not is taken token by token whatever its length, half a microsecond a token; copy it first.
     A value that is not finite reaches what it reaches in the recurrence, never an earlier token: a (request, head) whose
     new state is not finite is taken again token by token (half a microsecond a token). `out` shares no memory with q, k,
     v, g or beta."""

@@ -99,3 +99,18 @@ def test_gdn_chunked_overflows_as_the_recurrence_does(what, value):
             assert bool(((x - y).abs() <= 2 * HALF_BF16 * y.abs() + 2.0 ** -12 * y.abs().max()).all())
     fin = b["state"].isfinite()
     assert torch.equal(a["state"].isfinite(), fin)
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v", "out"])
+def test_gdn_chunked_long_run_off_the_boundaries(which):
+    """A long run with one operand off 16-byte boundaries goes token by token: the same recurrence."""
+    a = _inputs([700, 300], 2, 4, seed=3)
+    out, pool = _definition(a)
+    shift = lambda x: torch.empty(x.numel() + 1, dtype=torch.bfloat16, device=DEV)[1:].view(x.shape)  # noqa: E731
+    if which == "out":
+        got = G.gdn_chunked(**a, out=shift(a["v"]))
+    else:
+        got = G.gdn_chunked(**{**a, which: shift(a[which]).copy_(a[which])})
+    # one bf16 rounding; sums of 128 products in fp32 over a memory of some ten tokens stay below 2^-13 of the largest value
+    assert bool(((got.double() - out).abs() <= HALF_BF16 * out.abs() + 2.0 ** -13 * out.abs().max()).all())
+    assert bool(((a["state"].double() - pool).abs() <= 2.0 ** -14 * pool.abs().max()).all())
