@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(128, 4) gdn_prep_kernel(const GdnArgs a, uint8
 // finite in k, v, g, beta, X or S makes V' so, and through it the state, which stays so: if an element of the last state
 // is not finite, the state warps take the request's tokens one by one from the state in memory, which is written only at
 // the end. A q that is not finite reaches its own token's outputs alone.
-// Measured: 2.57 us a chunk (128 chunks of 8 heads in 329 us), 2.2 of them before R and V' c2 got their third pieces; the
+// Measured: 2.62 us a chunk (128 chunks of 8 heads in 336 us), 2.2 of them before R and V' c2 got their third pieces; the
 // tensor core is busy for 1.2 us of it (a product with A in TMEM costs N / 2 cycles), the state warps' conversions for 1.
 // One waiting lane at the issuer, all waits with a timer, one lane per value column in every token: 3.9 us. Requests in
 // order of length, the longest first: 250 instead of 260 us for 48 requests of 16384 tokens, lost again on ordering them.

@@ -53,7 +53,8 @@ class ModelConfig:
     gdn_value_dim: int = 128
     gdn_conv_kernel: int = 4
     # prompt passes of the GDN layers: "recurrent" (token by token) or "chunked" (64 tokens at a time on the tensor core:
-    # the same recurrence, rounded in other places; 12 to 18 times as fast on passes of thousands of tokens)
+    # the same recurrence, rounded in other places; 5 to 19 times as fast on passes of thousands of tokens: 64 short
+    # requests x 16 heads 0.52 to 0.65 -> 0.11 ms, one of 8192 tokens x 8 heads 6.75 -> 0.36)
     gdn_prefill: str = "recurrent"
     # RMS norm of every query and key head (weights [head_dim] per layer) before the rotation
     qk_norm: bool = False
@@ -115,6 +116,8 @@ class SpecConfig:
     benchmark configs (random-init weights never agree with their draft otherwise). "rejection" (chain mode): drafts
     are sampled from the drafter's distribution under the request's sampling parameters and verified by rejection
     against it, so that the emitted tokens follow the target's distribution exactly; greedy requests as under "exact".
+    The drafter needs the target's vocabulary. A step forms dense distributions: 64 requests x 4 drafts x 128256 tokens
+    cost 11.7 ms where "exact" takes 0.3.
     """
 
     enabled: bool = True
